@@ -12,8 +12,11 @@ from importlib import import_module
 
 _EXPORTS = {
     "BatchMLADecodeCuteDSLFP4Wrapper": ".wrapper",
+    "BatchMLASparseDecodeFP4Wrapper": ".sparse",
     "FP4MLADecodeBackend": ".adapter",
     "FP4MLAPagedCache": ".adapter",
+    "FP4MLAPagePool": ".pages",
+    "SparsePages": ".sparse",
     "decode_slot_mapping": ".adapter",
     "StandardAttention": ".variants",
     "AttentionWithSink": ".variants",

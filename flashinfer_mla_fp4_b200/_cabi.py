@@ -86,10 +86,61 @@ EXPORTS = (
     "mla_fp4_cp_free",
     "mla_fp4_cp_exchange_merge",
     "mla_fp4_step_metadata",
+    "mla_fp4_summarize_pages",
+    "mla_fp4_summarize_new_pages",
+    "mla_fp4_select_workspace_bytes",
+    "mla_fp4_select_pages",
+    "mla_fp4_pool_workspace_bytes",
+    "mla_fp4_copy_pages",
+    "mla_fp4_pool_allocate",
+    "mla_fp4_pool_fork",
+    "mla_fp4_pool_free",
+    "mla_fp4_pool_compact",
 )
 CP_MAX_RANKS = 8
 CP_HANDLE_BYTES = 64
 CP_AUTO, CP_ALL_GATHER, CP_REDUCE_SCATTER = 0, 1, 2
+
+
+class SelectArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_stride_batch", C.c_int64), ("q_stride_qpos", C.c_int64), ("q_stride_head", C.c_int64),
+        ("summary", C.c_void_p), ("summary_sf", C.c_void_p),
+        ("num_pages", C.c_int64),
+        ("block_tables", C.c_void_p), ("block_table_stride", C.c_int64),
+        ("seq_lens", C.c_void_p),
+        ("selected", C.c_void_p), ("selected_lens", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("batch", C.c_int32), ("q_len", C.c_int32), ("num_heads", C.c_int32), ("page_size", C.c_int32),
+        ("width", C.c_int32),
+        ("budget", C.c_int32), ("sink_pages", C.c_int32), ("local_pages", C.c_int32),
+        ("causal", C.c_int32),
+        ("reserved", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PageLayer(C.Structure):
+    _fields_ = [("kv_cache", C.c_void_p), ("kv_cache_sf", C.c_void_p), ("summary", C.c_void_p), ("summary_sf", C.c_void_p)]
+
+
+class PoolArgs(C.Structure):
+    _fields_ = [
+        ("layers", C.POINTER(PageLayer)),
+        ("num_layers", C.c_int32), ("page_size", C.c_int32),
+        ("num_pages", C.c_int64),
+        ("refcounts", C.c_void_p),
+        ("block_tables", C.c_void_p), ("block_table_stride", C.c_int64),
+        ("width", C.c_int32), ("rows", C.c_int32),
+        ("seq_lens", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("status", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+POOL_BAD_ROW, POOL_OUT_OF_PAGES = 1, 2
 
 
 def _load() -> C.CDLL:
@@ -145,6 +196,21 @@ def _load() -> C.CDLL:
     lib.mla_fp4_step_metadata.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,
                                           C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]
     lib.mla_fp4_step_metadata.restype = C.c_int
+    vp, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
+    for name, args in {
+        "mla_fp4_summarize_pages": [vp, vp, i64, i32, vp, i64, vp, vp, vp],
+        "mla_fp4_summarize_new_pages": [vp, vp, i64, i32, vp, i64, i32, vp, i32, i32, vp, vp, vp],
+        "mla_fp4_select_workspace_bytes": [i32, i32, i32, C.POINTER(C.c_size_t)],
+        "mla_fp4_select_pages": [C.POINTER(SelectArgs)],
+        "mla_fp4_pool_workspace_bytes": [i64, i32, i32, C.POINTER(C.c_size_t)],
+        "mla_fp4_copy_pages": [C.POINTER(PageLayer), i32, i64, i32, vp, vp, i64, vp],
+        "mla_fp4_pool_allocate": [C.POINTER(PoolArgs), vp],
+        "mla_fp4_pool_fork": [C.POINTER(PoolArgs), vp, vp, i32],
+        "mla_fp4_pool_free": [C.POINTER(PoolArgs), vp, i32],
+        "mla_fp4_pool_compact": [C.POINTER(PoolArgs), vp],
+    }.items():
+        fn = getattr(lib, name)
+        fn.argtypes, fn.restype = args, C.c_int
     v = lib.mla_fp4_abi_version()
     if v != ABI_VERSION:
         raise ImportError(f"{LIB_PATH} has ABI version {v}, expected {ABI_VERSION}: rebuild it")
@@ -193,4 +259,16 @@ def workspace_init(ptr: int, nbytes: int, stream: int) -> None:
 def workspace_bytes(batch: int, q_len: int, num_heads: int, num_ctas: int) -> int:
     out = C.c_size_t(0)
     check(lib.mla_fp4_workspace_bytes(batch, q_len, num_heads, num_ctas, C.byref(out)))
+    return int(out.value)
+
+
+def select_workspace_bytes(batch: int, q_len: int, width: int) -> int:
+    out = C.c_size_t(0)
+    check(lib.mla_fp4_select_workspace_bytes(batch, q_len, width, C.byref(out)))
+    return int(out.value)
+
+
+def pool_workspace_bytes(num_pages: int, rows: int, count: int) -> int:
+    out = C.c_size_t(0)
+    check(lib.mla_fp4_pool_workspace_bytes(num_pages, rows, count, C.byref(out)))
     return int(out.value)

@@ -5,7 +5,7 @@ handling, and SGLang backend routing remain the caller's responsibility" (refere
 README.md:81-83) and its serving integration is private (README.md:124-126).  This module is
 that caller for the decode step, in the shape paged-attention backends have:
 
-* ``FP4MLAPagedCache``        the two cache tensors of the format (rows + per-token scales);
+* ``FP4MLAPagedCache``        the two cache tensors of the format (rows + per-token scales), and the pages' summaries for sparse decode;
 * ``decode_slot_mapping``     flat cache slots of the tokens a decode step appends;
 * ``FP4MLADecodeBackend``     persistent (CUDA-graph-safe) step metadata, ``prepare()`` to
   refresh it from the scheduler's tensors, ``forward()`` = append the step's tokens to the cache
@@ -23,23 +23,47 @@ import torch
 
 from .api_log import api_logged
 from .kvcache import HEAD_DIM_QK, LATENT_DIM, ROPE_DIM, ROW_BYTES, write_tokens
+from .sparse import BatchMLASparseDecodeFP4Wrapper, SparsePages, summarize_new_pages
 from .wrapper import BatchMLADecodeCuteDSLFP4Wrapper
 
 
 class FP4MLAPagedCache:
-    """The paged cache of one layer: ``kv_cache`` u8 [pages, page_size, 320] and ``kv_cache_sf`` f32 [pages, page_size, 1]."""
+    """The paged cache of one layer: ``kv_cache`` u8 [pages, page_size, 320] and ``kv_cache_sf`` f32 [pages, page_size, 1].
 
-    def __init__(self, num_pages: int, page_size: int, device) -> None:
+    With ``summaries`` also what sparse decode selects pages by (``sparse.summarize_pages``): ``summary`` int8 [pages, 576] and ``summary_sf``
+    f32 [pages]; None without."""
+
+    def __init__(self, num_pages: int, page_size: int, device, summaries: bool = False) -> None:
         self.page_size = page_size
         self.kv_cache = torch.zeros(num_pages, page_size, ROW_BYTES, dtype=torch.uint8, device=device)
         self.kv_cache_sf = torch.zeros(num_pages, page_size, 1, dtype=torch.float32, device=device)
+        self.summary = torch.zeros(num_pages, HEAD_DIM_QK, dtype=torch.int8, device=device) if summaries else None
+        self.summary_sf = torch.zeros(num_pages, dtype=torch.float32, device=device) if summaries else None
+
+    @classmethod
+    def from_tensors(cls, kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summary: Optional[torch.Tensor] = None,
+                     summary_sf: Optional[torch.Tensor] = None) -> "FP4MLAPagedCache":
+        """A cache over tensors that the caller has (a layer of a larger allocation, say); nothing is copied."""
+        if kv_cache.dim() != 3 or kv_cache.shape[2] != ROW_BYTES or kv_cache.dtype != torch.uint8:
+            raise ValueError(f"kv_cache must be a uint8 tensor [pages, page_size, {ROW_BYTES}]")
+        if tuple(kv_cache_sf.shape) != (*kv_cache.shape[:2], 1) or kv_cache_sf.dtype != torch.float32:
+            raise ValueError("kv_cache_sf must be a float32 tensor [pages, page_size, 1]")
+        if (summary is None) != (summary_sf is None):
+            raise ValueError("summary and summary_sf belong together")
+        if summary is not None and (tuple(summary.shape) != (kv_cache.shape[0], HEAD_DIM_QK) or summary.dtype != torch.int8
+                                    or tuple(summary_sf.shape) != (kv_cache.shape[0],) or summary_sf.dtype != torch.float32):
+            raise ValueError(f"summary must be an int8 tensor [pages, {HEAD_DIM_QK}] and summary_sf a float32 tensor [pages]")
+        self = cls.__new__(cls)
+        self.page_size = kv_cache.shape[1]
+        self.kv_cache, self.kv_cache_sf, self.summary, self.summary_sf = kv_cache, kv_cache_sf, summary, summary_sf
+        return self
 
     @property
     def num_pages(self) -> int:
         return self.kv_cache.shape[0]
 
     def bytes(self) -> int:
-        return self.kv_cache.numel() + 4 * self.kv_cache_sf.numel()
+        return self.kv_cache.numel() + 4 * self.kv_cache_sf.numel() + (0 if self.summary is None else (HEAD_DIM_QK + 4) * self.num_pages)
 
 
 def decode_slot_mapping(block_tables: torch.Tensor, seq_lens: torch.Tensor, page_size: int, q_len: int = 1) -> torch.Tensor:
@@ -72,24 +96,37 @@ class FP4MLADecodeBackend:
 
     def __init__(self, num_heads: int, page_size: int, max_batch: int, max_seq_len: int, softmax_scale: float, device,
                  *, q_len: int = 1, out_dtype: Optional[torch.dtype] = None, output_scale: float = 1.0,
-                 workspace_buffer: Optional[torch.Tensor] = None, cp_group=None) -> None:
+                 workspace_buffer: Optional[torch.Tensor] = None, cp_group=None, sparse: Optional[SparsePages] = None) -> None:
+        """``sparse`` (``sparse.SparsePages``): steps attend to the pages that each query position selects; the caches need summaries, and
+        ``forward()`` keeps those of the pages that its tokens fill (those of prompts are written with ``sparse.summarize_new_pages``)."""
         from . import _cabi
 
+        if sparse is not None and cp_group is not None:
+            raise ValueError("sparse decode has no context-parallel form: a rank sees the pages of its own share alone")
         self.device = torch.device(device)
         self.num_heads, self.page_size, self.q_len = num_heads, page_size, q_len
         self.max_batch, self.max_seq_len = max_batch, max_seq_len
         self.softmax_scale, self.output_scale = float(softmax_scale), float(output_scale)
+        self.max_pages = (max_seq_len + page_size - 1) // page_size
+        self.sparse = sparse
         if workspace_buffer is None:
             sms = torch.cuda.get_device_properties(self.device).multi_processor_count
-            workspace_buffer = torch.empty(_cabi.workspace_bytes(max_batch, q_len, num_heads, sms), dtype=torch.int8, device=self.device)
-        self.wrapper = BatchMLADecodeCuteDSLFP4Wrapper(workspace_buffer)
-        self.wrapper.plan(num_heads=num_heads, page_size=page_size, out_dtype=out_dtype)
+            need = (_cabi.workspace_bytes(max_batch, q_len, num_heads, sms) if sparse is None else
+                    BatchMLASparseDecodeFP4Wrapper.workspace_bytes(max_batch, q_len, num_heads, self.max_pages, sparse.budget_pages, sms))
+            workspace_buffer = torch.empty(need, dtype=torch.int8, device=self.device)
+        if sparse is None:
+            self.wrapper = BatchMLADecodeCuteDSLFP4Wrapper(workspace_buffer)
+            self.wrapper.plan(num_heads=num_heads, page_size=page_size, out_dtype=out_dtype)
+        else:
+            self.wrapper = BatchMLASparseDecodeFP4Wrapper(workspace_buffer)
+            self.wrapper.plan(num_heads=num_heads, page_size=page_size, budget_pages=sparse.budget_pages, sink_pages=sparse.sink_pages,
+                              local_pages=sparse.local_pages, causal=sparse.causal, out_dtype=out_dtype)
+        self._out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
         self._runner = self.wrapper
         if cp_group is not None:
             from .distributed import ContextParallelDecoder
 
             self._runner = ContextParallelDecoder(self.wrapper, cp_group, max_rows=max_batch * q_len * num_heads)
-        self.max_pages = (max_seq_len + page_size - 1) // page_size
         self.block_tables = torch.zeros(max_batch, self.max_pages, dtype=torch.int32, device=self.device)
         self.seq_lens = torch.zeros(max_batch, dtype=torch.int32, device=self.device)
         self.slot_mapping = torch.full((max_batch * q_len,), -1, dtype=torch.int64, device=self.device)
@@ -155,7 +192,7 @@ class FP4MLADecodeBackend:
         positions (the reference itself accepts only ``q_len`` = 1, wrappers/batch_mla_fp4.py:297-298).  That is
         the attention of a batched multi-token step whose positions may see one another; a verification step of
         speculative decoding that needs position i blind to positions > i must issue its positions as separate
-        requests (``q_len`` = 1, ``seq_len`` reduced accordingly).
+        requests (``q_len`` = 1, ``seq_len`` reduced accordingly).  A backend with ``SparsePages(causal=True)`` has that mask.
         """
         batch = q.shape[0]
         if batch > self.max_batch or q.shape[1] != self.q_len:
@@ -165,6 +202,8 @@ class FP4MLADecodeBackend:
             raise ValueError(f"latent must be [{n}, {LATENT_DIM}] and rope [{n}, {ROPE_DIM}]")
         if cache.page_size != self.page_size:
             raise ValueError(f"cache page size {cache.page_size} does not match the backend's {self.page_size}")
+        if self.sparse is not None and cache.summary is None:
+            raise ValueError("sparse decode needs a cache with summaries (FP4MLAPagedCache(..., summaries=True))")
         bt, sl, sm = self.block_tables, self.seq_lens, self.slot_mapping
         views = self._views  # one attribute read: a batch and the rows of the same batch, whatever another thread does
         if views[0] != batch or views[4] is not bt or views[5] is not sl or views[6] is not sm:
@@ -173,6 +212,10 @@ class FP4MLADecodeBackend:
         longest = self._longest
         if longest != self.max_seq_len and torch.cuda.is_current_stream_capturing():  # (the graph is for other steps than this one)
             longest = self._longest_captured
+        if self.sparse is not None:
+            summarize_new_pages(cache.kv_cache, cache.kv_cache_sf, cache.summary, cache.summary_sf, views[1], views[2], self.q_len)
+            return self._runner.run(q, cache.kv_cache, views[1], views[2], longest, self.softmax_scale, output_scale=self.output_scale,
+                                    out=out, kv_cache_sf=cache.kv_cache_sf, summary=cache.summary, summary_sf=cache.summary_sf)
         return self._runner.run(q, cache.kv_cache, views[1], views[2], longest, self.softmax_scale,
                                 output_scale=self.output_scale, out=out, kv_cache_sf=cache.kv_cache_sf)
 
@@ -197,7 +240,7 @@ class FP4MLADecodeBackend:
         step.q = torch.zeros(batch, self.q_len, self.num_heads, HEAD_DIM_QK, dtype=torch.float8_e4m3fn, device=self.device)
         step.latent = torch.zeros(n, LATENT_DIM, dtype=in_dtype, device=self.device)
         step.rope = torch.zeros(n, ROPE_DIM, dtype=in_dtype, device=self.device)
-        step.out = torch.empty(batch, self.q_len, self.num_heads, LATENT_DIM, dtype=self.wrapper._o_dtype, device=self.device)
+        step.out = torch.empty(batch, self.q_len, self.num_heads, LATENT_DIM, dtype=self._out_dtype, device=self.device)
         self.clear()
         if expected_seq_len is not None:
             self._longest = self._longest_captured = int(expected_seq_len)

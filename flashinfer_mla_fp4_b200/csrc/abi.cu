@@ -469,6 +469,181 @@ int mla_fp4_step_metadata(const int32_t* block_tables, int64_t block_table_strid
   return MLA_FP4_OK;
 }
 
+namespace {
+int summarize(mla::SummarizeParams& p, int64_t ctas, void* stream) {
+  if (!page_size_ok(p.page_size)) return fail(MLA_FP4_ERR_UNSUPPORTED, "page_size must be one of 8, 16, 32, 64, 128");
+  if (p.num_pages <= 0 || p.num_pages > INT_MAX) return fail(MLA_FP4_ERR_BAD_ARG, "num_pages out of range");
+  if (!p.kv_cache || !p.kv_cache_sf || !p.summary || !p.summary_sf) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  if (reinterpret_cast<uintptr_t>(p.kv_cache) % 16 || reinterpret_cast<uintptr_t>(p.summary) % 16) return fail(MLA_FP4_ERR_BAD_ARG, "kv_cache and summary must be 16-byte aligned");
+  if (ctas > INT_MAX) return fail(MLA_FP4_ERR_UNSUPPORTED, "too many pages in one call");
+  cudaError_t e = mla::launch_summarize(p, ctas, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(MLA_FP4_ERR_CUDA, std::string("summarize launch: ") + cudaGetErrorString(e));
+  return MLA_FP4_OK;
+}
+// the most tokens of a request, with room for arithmetic on them
+int table_cap(int width, int page_size) { return std::min(seq_cap_of(width, page_size), INT_MAX - 256); }
+}  // namespace
+
+int mla_fp4_summarize_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
+                            const int32_t* page_ids, int64_t count, void* summary, float* summary_sf, void* stream) {
+  if (count < 0) return fail(MLA_FP4_ERR_BAD_ARG, "count out of range");
+  if (count == 0) return MLA_FP4_OK;
+  if (!page_ids) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  mla::SummarizeParams p = {};
+  p.kv_cache = static_cast<const uint8_t*>(kv_cache); p.kv_cache_sf = kv_cache_sf;
+  p.summary = static_cast<int8_t*>(summary); p.summary_sf = summary_sf;
+  p.page_ids = page_ids; p.num_pages = num_pages; p.page_size = page_size;
+  return summarize(p, count, stream);
+}
+
+int mla_fp4_summarize_new_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
+                                const int32_t* block_tables, int64_t block_table_stride, int32_t width,
+                                const int32_t* seq_lens, int32_t batch, int32_t new_tokens, void* summary,
+                                float* summary_sf, void* stream) {
+  if (batch < 0 || width < 0 || new_tokens < 0) return fail(MLA_FP4_ERR_BAD_ARG, "batch/width/new_tokens out of range");
+  if (batch == 0 || width == 0 || new_tokens == 0) return MLA_FP4_OK;
+  if (!block_tables || !seq_lens) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  if (!page_size_ok(page_size)) return fail(MLA_FP4_ERR_UNSUPPORTED, "page_size must be one of 8, 16, 32, 64, 128");
+  mla::SummarizeParams p = {};
+  p.kv_cache = static_cast<const uint8_t*>(kv_cache); p.kv_cache_sf = kv_cache_sf;
+  p.summary = static_cast<int8_t*>(summary); p.summary_sf = summary_sf;
+  p.block_tables = block_tables; p.block_table_stride = block_table_stride; p.seq_lens = seq_lens;
+  p.num_pages = num_pages; p.page_size = page_size; p.new_tokens = new_tokens;
+  p.per_request = std::min(width, int32_t((int64_t(new_tokens) + page_size - 1) / page_size));
+  p.seq_cap = table_cap(width, page_size);
+  return summarize(p, int64_t(batch) * p.per_request, stream);
+}
+
+int mla_fp4_select_workspace_bytes(int32_t batch, int32_t q_len, int32_t width, size_t* bytes_out) {
+  if (!bytes_out || batch < 0 || q_len <= 0 || width < 0) return fail(MLA_FP4_ERR_BAD_ARG, "batch/q_len/width out of range");
+  *bytes_out = size_t(batch) * size_t(q_len) * size_t(width) * 4;
+  return MLA_FP4_OK;
+}
+
+int mla_fp4_select_pages(const MlaFp4SelectArgs* a) {
+  if (!a) return fail(MLA_FP4_ERR_BAD_ARG, "args is null");
+  if (a->batch < 0 || a->q_len <= 0 || a->num_heads <= 0 || a->width < 0) return fail(MLA_FP4_ERR_BAD_ARG, "batch/q_len/num_heads/width out of range");
+  if (a->num_heads > 128) return fail(MLA_FP4_ERR_UNSUPPORTED, "num_heads must be <= 128");
+  if (!page_size_ok(a->page_size)) return fail(MLA_FP4_ERR_UNSUPPORTED, "page_size must be one of 8, 16, 32, 64, 128");
+  if (a->sink_pages < 0 || a->local_pages < 1 || int64_t(a->sink_pages) + a->local_pages > a->budget)
+    return fail(MLA_FP4_ERR_BAD_ARG, "sink_pages must not be negative, local_pages at least 1, and their sum within the budget");
+  if (a->batch == 0) return MLA_FP4_OK;
+  if (int64_t(a->batch) * a->q_len > INT_MAX) return fail(MLA_FP4_ERR_UNSUPPORTED, "too many query positions");
+  if (!a->q || !a->summary || !a->summary_sf || !a->seq_lens || !a->selected || !a->selected_lens || (a->width > 0 && !a->block_tables))
+    return fail(MLA_FP4_ERR_BAD_ARG, "a required device pointer is null");
+  if (a->num_pages <= 0 || a->num_pages > INT_MAX) return fail(MLA_FP4_ERR_BAD_ARG, "num_pages out of range");
+  if (reinterpret_cast<uintptr_t>(a->q) % 16 || a->q_stride_head % 16 || a->q_stride_qpos % 16 || a->q_stride_batch % 16)
+    return fail(MLA_FP4_ERR_BAD_ARG, "q must be 16-byte aligned with strides that are multiples of 16");
+  if (reinterpret_cast<uintptr_t>(a->summary) % 16) return fail(MLA_FP4_ERR_BAD_ARG, "summary must be 16-byte aligned");
+  size_t need = 0;
+  mla_fp4_select_workspace_bytes(a->batch, a->q_len, a->width, &need);
+  if (a->width > a->budget && (!a->workspace || a->workspace_bytes < need)) {
+    char buf[160];
+    snprintf(buf, sizeof buf, "workspace has %zu bytes, but %zu are required", a->workspace ? a->workspace_bytes : size_t(0), need);
+    return fail(MLA_FP4_ERR_WORKSPACE_TOO_SMALL, buf);
+  }
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(MLA_FP4_ERR_BAD_ARG, "workspace must be 16-byte aligned");
+  mla::SelectParams p;
+  p.q = static_cast<const uint8_t*>(a->q);
+  p.q_stride_batch = a->q_stride_batch; p.q_stride_qpos = a->q_stride_qpos; p.q_stride_head = a->q_stride_head;
+  p.summary = static_cast<const int8_t*>(a->summary); p.summary_sf = a->summary_sf;
+  p.block_tables = a->block_tables; p.seq_lens = a->seq_lens;
+  p.selected = a->selected; p.selected_lens = a->selected_lens;
+  p.keys = static_cast<uint32_t*>(a->workspace);
+  p.block_table_stride = a->block_table_stride; p.num_pages = a->num_pages;
+  p.batch = a->batch; p.q_len = a->q_len; p.heads = a->num_heads; p.page_size = a->page_size; p.width = a->width;
+  p.budget = a->budget; p.sink = a->sink_pages; p.local = a->local_pages; p.causal = a->causal ? 1 : 0;
+  p.seq_cap = a->width > 0 ? table_cap(a->width, a->page_size) : 0;
+  cudaError_t e = mla::launch_select(p, reinterpret_cast<cudaStream_t>(a->stream));
+  if (e != cudaSuccess) return fail(MLA_FP4_ERR_CUDA, std::string("select launch: ") + cudaGetErrorString(e));
+  return MLA_FP4_OK;
+}
+
+namespace {
+int check_layers(const MlaFp4PageLayer* layers, int32_t n, int64_t num_pages, int32_t page_size) {
+  if (n <= 0 || !layers) return fail(MLA_FP4_ERR_BAD_ARG, "no layers");
+  if (!page_size_ok(page_size)) return fail(MLA_FP4_ERR_UNSUPPORTED, "page_size must be one of 8, 16, 32, 64, 128");
+  if (num_pages <= 0 || num_pages > INT_MAX / 2) return fail(MLA_FP4_ERR_BAD_ARG, "num_pages out of range");
+  for (int i = 0; i < n; ++i) {
+    const MlaFp4PageLayer& l = layers[i];
+    if (!l.kv_cache || !l.kv_cache_sf || !l.summary != !l.summary_sf) return fail(MLA_FP4_ERR_BAD_ARG, "a layer's pointer is null");
+    if (reinterpret_cast<uintptr_t>(l.kv_cache) % 16 || reinterpret_cast<uintptr_t>(l.kv_cache_sf) % 16 || reinterpret_cast<uintptr_t>(l.summary) % 16)
+      return fail(MLA_FP4_ERR_BAD_ARG, "a layer's caches must be 16-byte aligned");
+  }
+  static_assert(sizeof(MlaFp4PageLayer) == sizeof(mla::PageLayer), "layers are handed on as they are");
+  return MLA_FP4_OK;
+}
+const mla::PageLayer* layers_of(const MlaFp4PageLayer* l) { return reinterpret_cast<const mla::PageLayer*>(l); }
+int pool_params(const MlaFp4PoolArgs* a, int32_t count, mla::PoolParams* p) {
+  if (!a) return fail(MLA_FP4_ERR_BAD_ARG, "args is null");
+  if (int rc = check_layers(a->layers, a->num_layers, a->num_pages, a->page_size)) return rc;
+  if (count < 0 || a->width < 0 || a->rows < 0) return fail(MLA_FP4_ERR_BAD_ARG, "count/width/rows out of range");
+  if (!a->refcounts || (a->rows > 0 && (!a->seq_lens || (a->width > 0 && !a->block_tables)))) return fail(MLA_FP4_ERR_BAD_ARG, "a required device pointer is null");
+  size_t need = 0;
+  mla_fp4_pool_workspace_bytes(a->num_pages, a->rows, count, &need);
+  if (!a->workspace || a->workspace_bytes < need) {
+    char buf[160];
+    snprintf(buf, sizeof buf, "workspace has %zu bytes, but %zu are required", a->workspace ? a->workspace_bytes : size_t(0), need);
+    return fail(MLA_FP4_ERR_WORKSPACE_TOO_SMALL, buf);
+  }
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(MLA_FP4_ERR_BAD_ARG, "workspace must be 16-byte aligned");
+  p->refcounts = a->refcounts; p->block_tables = a->block_tables; p->seq_lens = a->seq_lens;
+  p->ws = static_cast<int32_t*>(a->workspace); p->status = a->status;
+  p->num_pages = a->num_pages; p->block_table_stride = a->block_table_stride;
+  p->page_size = a->page_size; p->width = a->width; p->rows = a->rows;
+  return MLA_FP4_OK;
+}
+int pool_launched(cudaError_t e) { return e == cudaSuccess ? MLA_FP4_OK : fail(MLA_FP4_ERR_CUDA, std::string("pool launch: ") + cudaGetErrorString(e)); }
+}  // namespace
+
+int mla_fp4_pool_workspace_bytes(int64_t num_pages, int32_t rows, int32_t count, size_t* bytes_out) {
+  if (!bytes_out || num_pages < 0 || rows < 0 || count < 0) return fail(MLA_FP4_ERR_BAD_ARG, "num_pages/rows/count out of range");
+  // a word or two per page (allocation, compaction), one per row and three per list entry (forking)
+  *bytes_out = 4 * (16 + 2 * size_t(num_pages) + size_t(rows) + 3 * size_t(count));
+  return MLA_FP4_OK;
+}
+
+int mla_fp4_copy_pages(const MlaFp4PageLayer* layers, int32_t num_layers, int64_t num_pages, int32_t page_size,
+                       const int32_t* src, const int32_t* dst, int64_t count, void* stream) {
+  if (int rc = check_layers(layers, num_layers, num_pages, page_size)) return rc;
+  if (count < 0) return fail(MLA_FP4_ERR_BAD_ARG, "count out of range");
+  if (count == 0) return MLA_FP4_OK;
+  if (!src || !dst) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  return pool_launched(mla::launch_copy_pages(layers_of(layers), num_layers, src, dst, count, num_pages, page_size, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int mla_fp4_pool_allocate(const MlaFp4PoolArgs* a, const int32_t* new_lens) {
+  mla::PoolParams p;
+  if (int rc = pool_params(a, 0, &p)) return rc;
+  if (p.rows == 0) return MLA_FP4_OK;
+  if (!new_lens) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  return pool_launched(mla::launch_pool_allocate(p, new_lens, reinterpret_cast<cudaStream_t>(a->stream)));
+}
+
+int mla_fp4_pool_fork(const MlaFp4PoolArgs* a, const int32_t* parents, const int32_t* children, int32_t count) {
+  mla::PoolParams p;
+  if (int rc = pool_params(a, count, &p)) return rc;
+  if (count == 0) return MLA_FP4_OK;
+  if (!parents || !children) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  if (int64_t(count) * (mla::kMaxLayers + 1) > INT_MAX) return fail(MLA_FP4_ERR_UNSUPPORTED, "too many forks in one call");
+  return pool_launched(mla::launch_pool_fork(p, layers_of(a->layers), a->num_layers, parents, children, count, reinterpret_cast<cudaStream_t>(a->stream)));
+}
+
+int mla_fp4_pool_free(const MlaFp4PoolArgs* a, const int32_t* rows, int32_t count) {
+  mla::PoolParams p;
+  if (int rc = pool_params(a, count, &p)) return rc;
+  if (count == 0) return MLA_FP4_OK;
+  if (!rows) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  return pool_launched(mla::launch_pool_free(p, rows, count, reinterpret_cast<cudaStream_t>(a->stream)));
+}
+
+int mla_fp4_pool_compact(const MlaFp4PoolArgs* a, int32_t* remap) {
+  mla::PoolParams p;
+  if (int rc = pool_params(a, 0, &p)) return rc;
+  if (!remap) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
+  return pool_launched(mla::launch_pool_compact(p, layers_of(a->layers), a->num_layers, remap, reinterpret_cast<cudaStream_t>(a->stream)));
+}
+
 int mla_fp4_dequant_e2m1_to_e4m3(const void* packed, void* out, int64_t n_bytes, void* stream) {
   if (n_bytes < 0 || (n_bytes % 4)) return fail(MLA_FP4_ERR_BAD_ARG, "n_bytes must be a non-negative multiple of 4");
   if (n_bytes == 0) return MLA_FP4_OK;

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/mla_fp4_b200.h"
+
 namespace mla {
 
 struct DecodeParams {
@@ -96,6 +98,64 @@ struct StepMetadataParams {
 };
 cudaError_t launch_step_metadata(const StepMetadataParams& p, cudaStream_t stream);
 cudaError_t launch_dequant(const void* in, void* out, int64_t n_bytes, cudaStream_t stream);
+// sparse.cu: either page_ids (one CTA each) or the block tables with the lengths (per_request CTAs per request)
+struct SummarizeParams {
+  const uint8_t* kv_cache;
+  const float* kv_cache_sf;
+  int8_t* summary;
+  float* summary_sf;
+  const int32_t* page_ids;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  int64_t block_table_stride, num_pages;
+  int32_t page_size, per_request, new_tokens;
+  int32_t seq_cap;  // as in DecodeParams
+};
+cudaError_t launch_summarize(const SummarizeParams& p, int64_t ctas, cudaStream_t stream);
+struct SelectParams {
+  const uint8_t* q;
+  int64_t q_stride_batch, q_stride_qpos, q_stride_head;
+  const int8_t* summary;
+  const float* summary_sf;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  int32_t* selected;       // [rows][budget]
+  int32_t* selected_lens;  // [rows]
+  uint32_t* keys;          // workspace: [rows][width]
+  int64_t block_table_stride, num_pages;
+  int32_t batch, q_len, heads, page_size, width, budget, sink, local, causal;
+  int32_t seq_cap;  // as in DecodeParams
+};
+cudaError_t launch_select(const SelectParams& p, cudaStream_t stream);
+// pages.cu
+struct PageLayer {  // the caches of a layer; summary may be null
+  uint8_t* kv_cache;
+  float* kv_cache_sf;
+  int8_t* summary;
+  float* summary_sf;
+};
+constexpr int kMaxLayers = 64;  // in the parameters of a launch; more layers take more launches
+struct PageLayers {
+  PageLayer layer[kMaxLayers];
+  int32_t count;
+};
+constexpr int kPoolBadRow = MLA_FP4_POOL_BAD_ROW, kPoolOutOfPages = MLA_FP4_POOL_OUT_OF_PAGES;
+struct PoolParams {
+  int32_t* refcounts;
+  int32_t* block_tables;
+  int32_t* seq_lens;
+  int32_t* ws;
+  int32_t* status;
+  int64_t num_pages, block_table_stride;
+  int32_t page_size, width, rows;
+};
+cudaError_t launch_copy_pages(const PageLayer* layers, int num_layers, const int32_t* src, const int32_t* dst, int64_t count, int64_t num_pages,
+                              int page_size, cudaStream_t stream);
+cudaError_t launch_pool_allocate(const PoolParams& p, const int32_t* new_lens, cudaStream_t stream);
+cudaError_t launch_pool_fork(const PoolParams& p, const PageLayer* layers, int num_layers, const int32_t* parents, const int32_t* children, int count,
+                             cudaStream_t stream);
+cudaError_t launch_pool_free(const PoolParams& p, const int32_t* rows, int count, cudaStream_t stream);
+cudaError_t launch_pool_compact(const PoolParams& p, const PageLayer* layers, int num_layers, int32_t* remap, cudaStream_t stream);
 // tcgen05 decode kernel (decode_sm100.cu). Returns cudaErrorNotSupported-like codes through `err`.
 cudaError_t launch_decode_sm100(const DecodeParams& p, int num_ctas, cudaStream_t stream, const char** err);
 

@@ -1,0 +1,351 @@
+// The care of a cache's pages: copying, allocation, forking and freeing of block-table rows, compaction of the pool.
+//
+// A pool has a reference count per page (0: free) and one or more layers, whose caches hold a page of the same number each: rows, scales
+// and, where there is one, the summary.  Which pages move is decided by one CTA from the counts and lengths in device memory (the host is
+// not asked, so every call can be captured); the next kernel moves them in every layer.  New pages are the free ones of the lowest
+// numbers, in the order in which they are asked for: the same calls give the same tables.
+#include <climits>
+
+#include "common.cuh"
+#include "launch.h"
+
+namespace mla {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kMoveThreads = 256;
+
+__device__ __forceinline__ void dependent_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// pages that `len` tokens take
+__device__ __forceinline__ int pages_of(int len, int page_size) { return len > 0 ? (len - 1) / page_size + 1 : 0; }
+__device__ __forceinline__ void report(int32_t* status, int code, int which) {
+  if (status) {
+    status[1] = which;
+    status[0] = code;
+  }
+}
+
+// Sum of the values of the CTA's threads before this one; *total: of all.  warp_s: a word per warp.
+template <typename T>
+__device__ __forceinline__ T scan_before(T v, T* warp_s, T* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  T sum = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T up = __shfl_up_sync(0xffffffffu, sum, o);
+    sum += lane >= o ? up : 0;
+  }
+  __syncthreads();
+  if (lane == 31) warp_s[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    T w = lane < warps ? warp_s[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const T up = __shfl_up_sync(0xffffffffu, w, o);
+      w += lane >= o ? up : 0;
+    }
+    warp_s[lane] = w;
+  }
+  __syncthreads();
+  *total = warp_s[warps - 1];
+  return sum - v + (warp ? warp_s[warp - 1] : 0);
+}
+
+// Calls take(number, page) for the free pages of the lowest numbers, the first `wanted` of them; returns how many there were.
+template <typename Take>
+__device__ __forceinline__ int for_free_pages(const int32_t* refcounts, int64_t num_pages, int wanted, int* warp_s, Take take) {
+  int found = 0;
+  for (int64_t base = 0; base < num_pages && found < wanted; base += kPlanThreads * 4) {
+    const int64_t at = base + threadIdx.x * 4;
+    bool free[4];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      free[i] = at + i < num_pages && refcounts[at + i] <= 0;
+      n += free[i];
+    }
+    int total, number = found + scan_before(n, warp_s, &total);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (free[i]) {
+        if (number < wanted) take(number, int(at + i));
+        ++number;
+      }
+    found += total;
+  }
+  return found < wanted ? found : wanted;
+}
+
+// ------------------------------------------------------------------------------------------ copying
+__device__ __forceinline__ void copy16(void* dst, const void* src, int n16) {
+  for (int i = threadIdx.x; i < n16; i += kMoveThreads) static_cast<uint4*>(dst)[i] = static_cast<const uint4*>(src)[i];
+}
+// page `from` of a layer to page `to` of it, by the whole CTA
+__device__ __forceinline__ void copy_page(const PageLayer& l, int page_size, int64_t from, int64_t to) {
+  const int64_t row = int64_t(page_size) * kRowBytes;
+  copy16(l.kv_cache + to * row, l.kv_cache + from * row, int(row / 16));
+  copy16(l.kv_cache_sf + to * page_size, l.kv_cache_sf + from * page_size, page_size / 4);
+  if (l.summary) {
+    copy16(l.summary + to * kQDim, l.summary + from * kQDim, kQDim / 16);
+    if (threadIdx.x == 0) l.summary_sf[to] = l.summary_sf[from];
+  }
+}
+
+__global__ void __launch_bounds__(kMoveThreads) copy_pages_kernel(const __grid_constant__ PageLayers ls, const int32_t* src, const int32_t* dst,
+                                                                  int64_t count, int64_t num_pages, int page_size) {
+  dependent_launch();
+  for (int64_t u = blockIdx.x; u < count * ls.count; u += gridDim.x) {
+    const int64_t i = u / ls.count;
+    const int64_t from = src[i], to = dst[i];
+    if (from >= 0 && from < num_pages && to >= 0 && to < num_pages && from != to) copy_page(ls.layer[u - i * ls.count], page_size, from, to);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ allocation
+__global__ void __launch_bounds__(kPlanThreads) allocate_kernel(PoolParams p, const int32_t* new_lens) {
+  __shared__ int warp_s[32];
+  __shared__ long long sum_s[32];
+  dependent_launch();
+  int32_t *offset = p.ws, *list = p.ws + p.rows;
+  long long total = 0;  // (rows may ask for more than 32 bits hold)
+  for (int base = 0; base < p.rows; base += kPlanThreads) {
+    const int r = base + threadIdx.x;
+    long long need = 0, sum;
+    if (r < p.rows) {
+      const int have = pages_of(p.seq_lens[r], p.page_size), want = pages_of(new_lens[r], p.page_size);
+      if (want > p.width) report(p.status, kPoolBadRow, r);
+      else if (want > have) need = want - have;
+    }
+    const long long at = total + scan_before(need, sum_s, &sum);
+    if (r < p.rows) offset[r] = int(min(at, (long long)(p.num_pages)));
+    total += sum;
+  }
+  const int found = for_free_pages(p.refcounts, p.num_pages, int(min(total, (long long)(p.num_pages))), warp_s, [&](int number, int page) { list[number] = page; });
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < p.rows; r += kPlanThreads / 32) {
+    const int have = pages_of(p.seq_lens[r], p.page_size), want = pages_of(new_lens[r], p.page_size), at = offset[r];
+    if (want > p.width || want <= have) continue;
+    if (at + want - have > found) {
+      if ((threadIdx.x & 31) == 0) report(p.status, kPoolOutOfPages, r);
+      continue;
+    }
+    for (int k = threadIdx.x & 31; k < want - have; k += 32) {
+      const int page = list[at + k];
+      p.block_tables[int64_t(r) * p.block_table_stride + have + k] = page;
+      p.refcounts[page] = 1;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ forking
+// Workspace: claim [rows], then for each fork its length (-1: it is not made), the page for its tail (-1: none) and, by number of
+// the tail, whose it is.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(PoolParams p, const int32_t* parents, const int32_t* children, int count) {
+  __shared__ int warp_s[32];
+  dependent_launch();
+  int32_t *claim = p.ws, *len_of = claim + p.rows, *tail_of = len_of + count, *owner = tail_of + count;
+  const auto in_table = [&](int r) { return r >= 0 && r < p.rows; };
+  for (int r = threadIdx.x; r < p.rows; r += kPlanThreads) claim[r] = INT_MAX;
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += kPlanThreads)
+    if (in_table(children[i]) && in_table(parents[i])) atomicMin(&claim[children[i]], i);
+  __syncthreads();
+  int tails = 0;
+  for (int base = 0; base < count; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int len = -1;
+    if (i < count && children[i] >= 0 && parents[i] >= 0) {  // (a negative row is padding)
+      if (in_table(children[i]) && in_table(parents[i]) && __ldcg(&claim[children[i]]) == i && p.seq_lens[children[i]] <= 0 &&
+          pages_of(p.seq_lens[parents[i]], p.page_size) <= p.width)
+        len = max(p.seq_lens[parents[i]], 0);
+      else
+        report(p.status, kPoolBadRow, i);
+    }
+    const int partial = len > 0 && len % p.page_size != 0;
+    int sum;
+    const int number = tails + scan_before(partial, warp_s, &sum);
+    if (i < count) {
+      len_of[i] = len;
+      tail_of[i] = -1;
+      if (partial) owner[number] = i;
+    }
+    tails += sum;
+  }
+  __syncthreads();
+  const int found = for_free_pages(p.refcounts, p.num_pages, tails, warp_s, [&](int number, int page) {
+    tail_of[owner[number]] = page;
+    p.refcounts[page] = 1;
+  });
+  __syncthreads();
+  for (int n = found + threadIdx.x; n < tails; n += kPlanThreads) {  // no page left for these tails
+    len_of[owner[n]] = -1;
+    report(p.status, kPoolOutOfPages, owner[n]);
+  }
+}
+
+// The first `count` CTAs write a row each, the others copy the tails, layer by layer.
+__global__ void __launch_bounds__(kMoveThreads) fork_kernel(PoolParams p, const __grid_constant__ PageLayers ls, const int32_t* parents,
+                                                            const int32_t* children, int count, bool with_rows) {
+  dependent_launch();
+  const int32_t *len_of = p.ws + p.rows, *tail_of = len_of + count;
+  if (with_rows && int(blockIdx.x) < count) {
+    const int i = blockIdx.x, len = len_of[i];
+    if (len < 0) return;
+    const int32_t* from = p.block_tables + int64_t(parents[i]) * p.block_table_stride;
+    int32_t* to = p.block_tables + int64_t(children[i]) * p.block_table_stride;
+    const int used = pages_of(len, p.page_size), full = len / p.page_size;
+    for (int k = threadIdx.x; k < used; k += kMoveThreads) {
+      int page = from[k];
+      if (k >= full) page = tail_of[i];
+      else if (page >= 0 && page < p.num_pages) atomicAdd(&p.refcounts[page], 1);
+      to[k] = page;
+    }
+    if (threadIdx.x == 0) p.seq_lens[children[i]] = len;
+    return;
+  }
+  const int u = int(blockIdx.x) - (with_rows ? count : 0), i = u / ls.count;
+  const int to = tail_of[i];
+  if (len_of[i] < 0 || to < 0) return;
+  const int from = p.block_tables[int64_t(parents[i]) * p.block_table_stride + len_of[i] / p.page_size];
+  if (from >= 0 && from < p.num_pages) copy_page(ls.layer[u - i * ls.count], p.page_size, from, to);
+}
+
+// ------------------------------------------------------------------------------------------ freeing
+__global__ void __launch_bounds__(kMoveThreads) free_kernel(PoolParams p, const int32_t* rows) {
+  __shared__ int len_s;
+  dependent_launch();
+  const int row = rows[blockIdx.x];
+  if (row < 0) return;  // padding
+  if (row >= p.rows) {
+    if (threadIdx.x == 0) report(p.status, kPoolBadRow, blockIdx.x);
+    return;
+  }
+  if (threadIdx.x == 0) len_s = atomicExch(&p.seq_lens[row], 0);  // a row that is named twice is freed once
+  __syncthreads();
+  const int used = min(pages_of(len_s, p.page_size), p.width);
+  for (int k = threadIdx.x; k < used; k += kMoveThreads) {
+    const int page = p.block_tables[int64_t(row) * p.block_table_stride + k];
+    if (page < 0 || page >= p.num_pages || atomicSub(&p.refcounts[page], 1) > 0) continue;
+    atomicAdd(&p.refcounts[page], 1);  // it was free already
+    report(p.status, kPoolBadRow, blockIdx.x);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ compaction
+// With n pages in use, the i-th of them whose number is n or more moves into the i-th free page below n.  Workspace: how many move, then
+// the holes, then the pages that move.
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PoolParams p, int32_t* remap) {
+  __shared__ int warp_s[32];
+  dependent_launch();
+  int32_t *hole = p.ws + 4, *high = hole + p.num_pages;
+  int mine = 0, live;
+  for (int64_t i = threadIdx.x; i < p.num_pages; i += kPlanThreads) mine += p.refcounts[i] > 0;
+  scan_before(mine, warp_s, &live);
+  int holes = 0, highs = 0;
+  for (int64_t base = 0; base < p.num_pages; base += kPlanThreads) {
+    const int64_t i = base + threadIdx.x;
+    const bool in = i < p.num_pages, used = in && p.refcounts[i] > 0;
+    const int a = in && !used && i < live, b = used && i >= live;
+    int sum;
+    const int before = scan_before(a | (b << 16), warp_s, &sum);
+    if (a) hole[holes + (before & 0xffff)] = int(i);
+    if (b) high[highs + (before >> 16)] = int(i);
+    if (in) remap[i] = used ? int(i) : -1;
+    holes += sum & 0xffff;
+    highs += sum >> 16;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < highs; i += kPlanThreads) {
+    const int from = high[i], to = hole[i];
+    remap[from] = to;
+    p.refcounts[to] = p.refcounts[from];
+    p.refcounts[from] = 0;
+  }
+  if (threadIdx.x == 0) p.ws[0] = highs;
+}
+
+// The first `rows` CTAs (with_rows) rewrite a block-table row each, the others copy.
+__global__ void __launch_bounds__(kMoveThreads) compact_kernel(PoolParams p, const __grid_constant__ PageLayers ls, const int32_t* remap, bool with_rows) {
+  dependent_launch();
+  const int first = with_rows ? p.rows : 0;
+  if (int(blockIdx.x) < first) {
+    int32_t* row = p.block_tables + int64_t(blockIdx.x) * p.block_table_stride;
+    const int used = min(pages_of(p.seq_lens[blockIdx.x], p.page_size), p.width);
+    for (int k = threadIdx.x; k < used; k += kMoveThreads) {
+      const int page = row[k];
+      if (page >= 0 && page < p.num_pages && remap[page] >= 0) row[k] = remap[page];
+    }
+    return;
+  }
+  const int32_t *hole = p.ws + 4, *high = hole + p.num_pages;
+  const int64_t moves = int64_t(p.ws[0]) * ls.count;
+  for (int64_t u = int(blockIdx.x) - first; u < moves; u += int(gridDim.x) - first) {
+    const int64_t i = u / ls.count;
+    copy_page(ls.layer[u - i * ls.count], p.page_size, high[i], hole[i]);
+  }
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int threads, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Layers go kMaxLayers at a time; f(layers, whether these are the first) launches.
+template <typename F>
+cudaError_t by_layers(const PageLayer* layers, int count, F f) {
+  PageLayers ls;
+  for (int at = 0; at < count; at += kMaxLayers) {
+    ls.count = count - at < kMaxLayers ? count - at : kMaxLayers;
+    for (int i = 0; i < ls.count; ++i) ls.layer[i] = layers[at + i];
+    cudaError_t e = f(ls, at == 0);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+int64_t move_ctas(int64_t units) { return units < 148 * 64 ? units : 148 * 64; }
+
+}  // namespace
+
+cudaError_t launch_copy_pages(const PageLayer* layers, int num_layers, const int32_t* src, const int32_t* dst, int64_t count, int64_t num_pages,
+                              int page_size, cudaStream_t stream) {
+  return by_layers(layers, num_layers, [&](const PageLayers& ls, bool) {
+    return launch_dependent(copy_pages_kernel, move_ctas(count * ls.count), kMoveThreads, stream, ls, src, dst, count, num_pages, page_size);
+  });
+}
+cudaError_t launch_pool_allocate(const PoolParams& p, const int32_t* new_lens, cudaStream_t stream) {
+  return launch_dependent(allocate_kernel, 1, kPlanThreads, stream, p, new_lens);
+}
+cudaError_t launch_pool_fork(const PoolParams& p, const PageLayer* layers, int num_layers, const int32_t* parents, const int32_t* children, int count,
+                             cudaStream_t stream) {
+  cudaError_t e = launch_dependent(fork_plan_kernel, 1, kPlanThreads, stream, p, parents, children, count);
+  if (e != cudaSuccess) return e;
+  return by_layers(layers, num_layers, [&](const PageLayers& ls, bool first) {
+    return launch_dependent(fork_kernel, int64_t(count) * (ls.count + (first ? 1 : 0)), kMoveThreads, stream, p, ls, parents, children, count, first);
+  });
+}
+cudaError_t launch_pool_free(const PoolParams& p, const int32_t* rows, int count, cudaStream_t stream) {
+  return launch_dependent(free_kernel, count, kMoveThreads, stream, p, rows);
+}
+cudaError_t launch_pool_compact(const PoolParams& p, const PageLayer* layers, int num_layers, int32_t* remap, cudaStream_t stream) {
+  cudaError_t e = launch_dependent(compact_plan_kernel, 1, kPlanThreads, stream, p, remap);
+  if (e != cudaSuccess) return e;
+  return by_layers(layers, num_layers, [&](const PageLayers& ls, bool first) {
+    return launch_dependent(compact_kernel, (first ? p.rows : 0) + move_ctas(p.num_pages / 2 * ls.count + 1), kMoveThreads, stream, p, ls, remap, first);
+  });
+}
+
+}  // namespace mla

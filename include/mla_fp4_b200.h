@@ -276,6 +276,102 @@ int mla_fp4_step_metadata(const int32_t* block_tables, int64_t block_table_strid
                           int32_t q_len, int32_t* dst_block_tables, int64_t dst_block_table_stride,
                           int32_t* dst_seq_lens, int64_t* dst_slot_mapping, int32_t max_batch, void* stream);
 
+/* Sparse decode over pages that a cheap score selects (no counterpart in the reference).  A page's summary is its mean key in
+   8 bits: summary int8 [num_pages][576] (16-byte aligned) and summary_sf f32 [num_pages].  With S = max |s_t| over the page's n
+   token scales and w_t = round(32767 s_t / S): the latent mean is S / (32767 n) sum_t w_t e_td (e: E2M1 values), the
+   RoPE mean 1/n sum_t r_td, scale = max |mean| / 127 (to FP32), code = round(mean / scale).  A page with a token scale that is
+   not finite or a NaN among its RoPE values gets the scale NaN.  Only full pages are ever scored.
+     mla_fp4_summarize_pages: of page_ids int32 [count]; ids outside the pool are skipped.
+     mla_fp4_summarize_new_pages: of the pages that the last new_tokens positions of each request have filled (seq_lens counts them):
+       what a step calls behind mla_fp4_cache_write.  width is that of a block-table row in pages.
+   Asynchronous on `stream`, nothing allocated. */
+int mla_fp4_summarize_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
+                            const int32_t* page_ids, int64_t count, void* summary, float* summary_sf, void* stream);
+int mla_fp4_summarize_new_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
+                                const int32_t* block_tables, int64_t block_table_stride, int32_t width,
+                                const int32_t* seq_lens, int32_t batch, int32_t new_tokens, void* summary,
+                                float* summary_sf, void* stream);
+
+/* Selection: for every query position (row = request * q_len + position) the pages it attends to, as a block table int32
+   [rows][budget] and lengths int32 [rows] for mla_fp4_decode with batch = rows, q_len = 1.  Of a request with no more than
+   `budget` pages all; of a longer one the first sink_pages, the last local_pages (at least one: the page that is not
+   full is among them) and the best of the rest, in the order of the request.  Entries behind the last page are 0.
+   The score of a page is summary_sf * max_h 2^-k_h <q_h, code> with q_h = round(q 2^k_h), k_h bringing the largest binade of
+   head h to [64, 128), one rounding to FP32 at the end; NaN bytes of q count as zero.  NaN scores come first, ties go to
+   the page nearer the start, pages outside the pool come last.
+   causal != 0: position i of q_len does not see the q_len - 1 - i newest tokens.
+   The pages are the same on every GPU and run: dots are of integers. */
+typedef struct MlaFp4SelectArgs {
+  const void* q;  /* as in MlaFp4DecodeArgs: E4M3, strides in bytes, 16-byte aligned */
+  int64_t q_stride_batch, q_stride_qpos, q_stride_head;
+  const void* summary;
+  const float* summary_sf;
+  int64_t num_pages;
+  const int32_t* block_tables;
+  int64_t block_table_stride;
+  const int32_t* seq_lens;
+  int32_t* selected;       /* [batch * q_len][budget] */
+  int32_t* selected_lens;  /* [batch * q_len] */
+  void* workspace;         /* mla_fp4_select_workspace_bytes; 16-byte aligned; nothing is kept in it */
+  size_t workspace_bytes;
+  int32_t batch, q_len, num_heads, page_size;
+  int32_t width;           /* pages per block-table row; lengths beyond width * page_size are cut to it */
+  int32_t budget, sink_pages, local_pages;
+  int32_t causal;
+  int32_t reserved;        /* 0 */
+  void* stream;
+} MlaFp4SelectArgs;
+int mla_fp4_select_workspace_bytes(int32_t batch, int32_t q_len, int32_t width, size_t* bytes_out);
+int mla_fp4_select_pages(const MlaFp4SelectArgs* args);
+
+/* The care of a cache's pages (no counterpart in the reference).  A pool is the caches of one or more layers, which hold a page
+   of the same number each, with one reference count per page: refcounts int32 [num_pages] on the device, 0 = free.
+   block_tables int32 [rows][block_table_stride] and seq_lens int32 [rows] (tokens that a row holds) are on the device too, and so are
+   the lists of rows and pages; negative entries of a list are padding.  Every call is asynchronous on `stream` and
+   allocates nothing; what it decides it decides on the device.  New pages are the free ones of the lowest numbers, in the order in which they
+   are asked for.
+     mla_fp4_copy_pages: page src[i] to page dst[i] in every layer, i < count; pairs with a page outside the pool are skipped.  No page
+       may be named twice among dst, or both in src and in dst: the copies run at once.
+     mla_fp4_pool_allocate: pages for the rows that are to hold new_lens [rows] tokens and have those for seq_lens.  seq_lens stays as
+       it is.  Rows are served in order; one that does not fit any more, or not into its block-table row, gets none.
+     mla_fp4_pool_fork: row children[i] (empty: length 0) becomes what row parents[i] is, i < count.  Full pages are shared, a last page that is
+       not full is copied in every layer.  A fork without a page for its tail, into a row that is not empty, or of a child named before, is not made.
+     mla_fp4_pool_free: the rows' pages lose a reference each, their lengths become 0.
+     mla_fp4_pool_compact: with n pages in use, the i-th of those numbered n or more moves into the i-th free one below n, in every layer;
+       counts and block tables follow, remap int32 [num_pages] says where each page went (-1: it was free).
+   status (int32 [8], may be NULL; zeroed by the caller) gets MLA_FP4_POOL_* in word 0 and the row or list entry in word 1 when a part of
+   a call was not done. */
+#define MLA_FP4_POOL_BAD_ROW 1
+#define MLA_FP4_POOL_OUT_OF_PAGES 2
+typedef struct MlaFp4PageLayer {
+  void* kv_cache;     /* [num_pages][page_size][320], 16-byte aligned */
+  float* kv_cache_sf; /* [num_pages][page_size], 16-byte aligned */
+  void* summary;      /* [num_pages][576], 16-byte aligned, or NULL */
+  float* summary_sf;  /* [num_pages] or NULL with it */
+} MlaFp4PageLayer;
+typedef struct MlaFp4PoolArgs {
+  const MlaFp4PageLayer* layers; /* on the host */
+  int32_t num_layers, page_size;
+  int64_t num_pages;
+  int32_t* refcounts;
+  int32_t* block_tables;
+  int64_t block_table_stride;
+  int32_t width, rows;
+  int32_t* seq_lens;
+  void* workspace; /* mla_fp4_pool_workspace_bytes; 4-byte aligned; nothing is kept in it */
+  size_t workspace_bytes;
+  int32_t* status;
+  void* stream;
+} MlaFp4PoolArgs;
+/* for calls with that many rows, and lists of that many entries */
+int mla_fp4_pool_workspace_bytes(int64_t num_pages, int32_t rows, int32_t count, size_t* bytes_out);
+int mla_fp4_copy_pages(const MlaFp4PageLayer* layers, int32_t num_layers, int64_t num_pages, int32_t page_size,
+                       const int32_t* src, const int32_t* dst, int64_t count, void* stream);
+int mla_fp4_pool_allocate(const MlaFp4PoolArgs* args, const int32_t* new_lens);
+int mla_fp4_pool_fork(const MlaFp4PoolArgs* args, const int32_t* parents, const int32_t* children, int32_t count);
+int mla_fp4_pool_free(const MlaFp4PoolArgs* args, const int32_t* rows, int32_t count);
+int mla_fp4_pool_compact(const MlaFp4PoolArgs* args, int32_t* remap);
+
 /* Largest decode grid the allocation-free variant below accepts, and the bytes of device memory
    its built-in scratch occupies on every GPU that loads the library (until the process exits). */
 #define MLA_FP4_STATIC_MAX_CTAS 148
