@@ -116,7 +116,8 @@ class SelectArgs(C.Structure):
         ("width", C.c_int32),
         ("budget", C.c_int32), ("sink_pages", C.c_int32), ("local_pages", C.c_int32),
         ("causal", C.c_int32),
-        ("reserved", C.c_int32),
+        ("wait_polls", C.c_int32),
+        ("status", C.c_void_p),
         ("stream", C.c_void_p),
     ]
 

@@ -527,6 +527,7 @@ int mla_fp4_select_pages(const MlaFp4SelectArgs* a) {
   if (!page_size_ok(a->page_size)) return fail(MLA_FP4_ERR_UNSUPPORTED, "page_size must be one of 8, 16, 32, 64, 128");
   if (a->sink_pages < 0 || a->local_pages < 1 || int64_t(a->sink_pages) + a->local_pages > a->budget)
     return fail(MLA_FP4_ERR_BAD_ARG, "sink_pages must not be negative, local_pages at least 1, and their sum within the budget");
+  if (a->wait_polls < 0) return fail(MLA_FP4_ERR_BAD_ARG, "wait_polls must not be negative");
   if (a->batch == 0) return MLA_FP4_OK;
   if (int64_t(a->batch) * a->q_len > INT_MAX) return fail(MLA_FP4_ERR_UNSUPPORTED, "too many query positions");
   if (!a->q || !a->summary || !a->summary_sf || !a->seq_lens || !a->selected || !a->selected_lens || (a->width > 0 && !a->block_tables))
@@ -554,7 +555,11 @@ int mla_fp4_select_pages(const MlaFp4SelectArgs* a) {
   p.batch = a->batch; p.q_len = a->q_len; p.heads = a->num_heads; p.page_size = a->page_size; p.width = a->width;
   p.budget = a->budget; p.sink = a->sink_pages; p.local = a->local_pages; p.causal = a->causal ? 1 : 0;
   p.seq_cap = a->width > 0 ? table_cap(a->width, a->page_size) : 0;
-  cudaError_t e = mla::launch_select(p, reinterpret_cast<cudaStream_t>(a->stream));
+  p.wait_polls = a->wait_polls > 0 ? uint32_t(a->wait_polls) : (1u << 22);
+  p.status = a->status;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  cudaError_t e = mla::launch_select(p, sms, reinterpret_cast<cudaStream_t>(a->stream));
   if (e != cudaSuccess) return fail(MLA_FP4_ERR_CUDA, std::string("select launch: ") + cudaGetErrorString(e));
   return MLA_FP4_OK;
 }

@@ -125,8 +125,11 @@ struct SelectParams {
   int64_t block_table_stride, num_pages;
   int32_t batch, q_len, heads, page_size, width, budget, sink, local, causal;
   int32_t seq_cap;  // as in DecodeParams
+  uint32_t wait_polls;
+  int32_t* status;
 };
-cudaError_t launch_select(const SelectParams& p, cudaStream_t stream);
+cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream);   // score_sm100.cu: the keys
+cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream);  // keys and selection
 // pages.cu
 struct PageLayer {  // the caches of a layer; summary may be null
   uint8_t* kv_cache;

@@ -6,8 +6,7 @@
 // numbers, in the order in which they are asked for: the same calls give the same tables.
 #include <climits>
 
-#include "common.cuh"
-#include "launch.h"
+#include "sparse.cuh"
 
 namespace mla {
 
@@ -16,10 +15,6 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kMoveThreads = 256;
 
-__device__ __forceinline__ void dependent_launch() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
 // pages that `len` tokens take
 __device__ __forceinline__ int pages_of(int len, int page_size) { return len > 0 ? (len - 1) / page_size + 1 : 0; }
 __device__ __forceinline__ void report(int32_t* status, int code, int which) {
@@ -291,17 +286,8 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(PoolParams p, con
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int threads, cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(grid));
-  cfg.blockDim = dim3(threads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+cudaError_t launch_pool(void (*kernel)(Params...), int64_t grid, int threads, cudaStream_t stream, const Args&... args) {
+  return launch_dependent(kernel, dim3(unsigned(grid)), threads, 0, stream, args...);
 }
 
 // Layers go kMaxLayers at a time; f(layers, whether these are the first) launches.
@@ -323,28 +309,28 @@ int64_t move_ctas(int64_t units) { return units < 148 * 64 ? units : 148 * 64; }
 cudaError_t launch_copy_pages(const PageLayer* layers, int num_layers, const int32_t* src, const int32_t* dst, int64_t count, int64_t num_pages,
                               int page_size, cudaStream_t stream) {
   return by_layers(layers, num_layers, [&](const PageLayers& ls, bool) {
-    return launch_dependent(copy_pages_kernel, move_ctas(count * ls.count), kMoveThreads, stream, ls, src, dst, count, num_pages, page_size);
+    return launch_pool(copy_pages_kernel, move_ctas(count * ls.count), kMoveThreads, stream, ls, src, dst, count, num_pages, page_size);
   });
 }
 cudaError_t launch_pool_allocate(const PoolParams& p, const int32_t* new_lens, cudaStream_t stream) {
-  return launch_dependent(allocate_kernel, 1, kPlanThreads, stream, p, new_lens);
+  return launch_pool(allocate_kernel, 1, kPlanThreads, stream, p, new_lens);
 }
 cudaError_t launch_pool_fork(const PoolParams& p, const PageLayer* layers, int num_layers, const int32_t* parents, const int32_t* children, int count,
                              cudaStream_t stream) {
-  cudaError_t e = launch_dependent(fork_plan_kernel, 1, kPlanThreads, stream, p, parents, children, count);
+  cudaError_t e = launch_pool(fork_plan_kernel, 1, kPlanThreads, stream, p, parents, children, count);
   if (e != cudaSuccess) return e;
   return by_layers(layers, num_layers, [&](const PageLayers& ls, bool first) {
-    return launch_dependent(fork_kernel, int64_t(count) * (ls.count + (first ? 1 : 0)), kMoveThreads, stream, p, ls, parents, children, count, first);
+    return launch_pool(fork_kernel, int64_t(count) * (ls.count + (first ? 1 : 0)), kMoveThreads, stream, p, ls, parents, children, count, first);
   });
 }
 cudaError_t launch_pool_free(const PoolParams& p, const int32_t* rows, int count, cudaStream_t stream) {
-  return launch_dependent(free_kernel, count, kMoveThreads, stream, p, rows);
+  return launch_pool(free_kernel, count, kMoveThreads, stream, p, rows);
 }
 cudaError_t launch_pool_compact(const PoolParams& p, const PageLayer* layers, int num_layers, int32_t* remap, cudaStream_t stream) {
-  cudaError_t e = launch_dependent(compact_plan_kernel, 1, kPlanThreads, stream, p, remap);
+  cudaError_t e = launch_pool(compact_plan_kernel, 1, kPlanThreads, stream, p, remap);
   if (e != cudaSuccess) return e;
   return by_layers(layers, num_layers, [&](const PageLayers& ls, bool first) {
-    return launch_dependent(compact_kernel, (first ? p.rows : 0) + move_ctas(p.num_pages / 2 * ls.count + 1), kMoveThreads, stream, p, ls, remap, first);
+    return launch_pool(compact_kernel, (first ? p.rows : 0) + move_ctas(p.num_pages / 2 * ls.count + 1), kMoveThreads, stream, p, ls, remap, first);
   });
 }
 

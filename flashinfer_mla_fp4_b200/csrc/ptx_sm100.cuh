@@ -169,6 +169,16 @@ MLA_UMMA_F8(umma_f8, "")
 MLA_UMMA_F8(umma_f8_a_fill, ".collector::a::fill")
 MLA_UMMA_F8(umma_f8_a_lastuse, ".collector::a::lastuse")
 #undef MLA_UMMA_F8
+// kind::i8: 8-bit integers, accumulated in 32 bits; predicated as umma_f8 is
+__device__ __forceinline__ void umma_i8(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
 // A value that is the same in all lanes of a converged warp, through a warp reduction: the compiler may then keep it, and
 // what is computed from it, in uniform registers.
 __device__ __forceinline__ uint32_t uniform_u32(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }

@@ -1,0 +1,372 @@
+// Scores of page summaries against queries (mathematics: sparse.cu) on the tensor cores: tcgen05.mma.kind::i8, 128 pages x heads x 576.
+//
+// Pages are the M axis: a thread of the epilogue has a page (a TMEM lane) and goes over its heads in registers; with the heads on M the
+// largest over heads would be a reduction across threads, and fewer than 128 heads would waste half of the MMA or more.
+//
+// Bound by HBM: a page's 580 bytes are read once per query position, an SM's share of the measured copy rate is a tile (128 pages, 74 KB) in
+// 1.7 us, and its 18 MMAs of 128 x 128 x 32 take less.  So a CTA per SM walks a contiguous range of the tiles of all rows, in two stages of a
+// whole tile each: at least one tile is in flight whatever the other roles do.  Rows come by cp.async straight into the
+// 64-byte swizzle of the operand (576 = 9 x 64 without a rest; eight rows x 64 bytes per instruction are one swizzle atom: no bank
+// conflicts, whole sectors); a TMA gather would take 288 instructions of 256 bytes a tile.
+//
+// Roles: warps 0-3 turn a row's query into integers (the B operand) and take the scores out of TMEM, warp 4 issues the MMAs, warps
+// 5-12 load.  All waits are bounded; one that runs out sets the status and ends the CTA, whose keys are then not all written.
+#include "common.cuh"
+#include "launch.h"
+#include "ptx_sm100.cuh"
+#include "sparse.cuh"
+
+namespace mla {
+
+namespace {
+
+constexpr int kEpiWarps = 4, kLoadWarps = 8;
+constexpr int kMmaWarp = kEpiWarps, kFirstLoad = kEpiWarps + 1;
+constexpr int kThreads = 32 * (kEpiWarps + 1 + kLoadWarps);
+constexpr int kPages = 128;                       // pages of a tile: the lanes of TMEM
+constexpr int kBlocks = kQDim / 64;               // 64-byte blocks of a summary
+constexpr int kStageBytes = kPages * kQDim;       // [9 blocks][128 pages][64 bytes], 64-byte swizzle
+constexpr int kStages = 2;
+constexpr int kMaxRows = 1024;                    // rows of a launch (the launcher makes several)
+constexpr uint32_t kTmemCols = 256;               // two accumulators of up to 128 columns
+
+// shared memory, from a 1024-byte boundary on: the stages, the query's codes [9][columns][64 bytes], then
+struct Small {
+  int candidates[kMaxRows];  // pages that a row scores
+  float unit[2][128];        // 2^-k of the heads, of the row in hand and the one before
+  unsigned long long full_a[kStages], empty_a[kStages], full_d[2], empty_d[2], full_b, drained;
+  uint32_t tmem;
+  int first_row, first_tile, tiles;  // of this CTA
+  volatile int abort;
+};
+
+__device__ __forceinline__ uint32_t bar(const unsigned long long& b) { return ptx::smem_u32(&b); }
+
+struct Ctx {
+  const SelectParams& p;
+  Small& s;
+};
+// Bounded: false when it ran out, here or in another role.
+__device__ __forceinline__ bool wait(const Ctx& c, const unsigned long long& b, uint32_t parity) {
+  for (uint32_t i = 0; i < c.p.wait_polls; ++i) {
+    if (ptx::mbar_try_wait(bar(b), parity)) return true;
+    if (c.s.abort) return false;
+  }
+  c.s.abort = 1;
+  if (c.p.status) {
+    c.p.status[1] = int(bar(b));
+    c.p.status[2] = blockIdx.x;
+    c.p.status[3] = threadIdx.x;
+    c.p.status[4] = int(parity);
+    c.p.status[0] = MLA_FP4_ERR_DEVICE_TIMEOUT;
+  }
+  return false;
+}
+
+// The tiles of a CTA in order, the same for every role.
+struct Walk {
+  const int* candidates;
+  int row, tile, left;
+  __device__ __forceinline__ Walk(const Small& s) : candidates(s.candidates), row(s.first_row), tile(s.first_tile), left(s.tiles) {}
+  __device__ __forceinline__ bool row_ends() const { return (tile + 1) * kPages >= candidates[row]; }
+  __device__ __forceinline__ int next_row() const {  // (there is one where tiles are left)
+    int r = row + 1;
+    while (candidates[r] == 0) ++r;
+    return r;
+  }
+  __device__ __forceinline__ void next() {
+    --left;
+    if (!row_ends()) ++tile;
+    else if (left > 0) row = next_row(), tile = 0;
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 b;\n\tcvt.u16.u32 b, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(two_bytes));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmax2_abs_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tand.b32 t, %2, 0x7fff7fff;\n\tmax.NaN.f16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// The heads of a row's query as integers, into shared memory: by the 128 threads of the epilogue, four lanes a head, 144 values each.  In FP16: an
+// E4M3 value times 2^k is exact, and adding 1536 rounds it to a whole number (to even, as round() does) that is the low byte of the sum.
+// Columns behind the last head repeat head 0, which leaves the largest score as it is.
+__device__ __forceinline__ void make_b(const SelectParams& p, char* b_smem, float* unit, int row, int columns) {
+  const int batch = row / p.q_len, tid = threadIdx.x;
+  const uint8_t* q = p.q + batch * p.q_stride_batch + (row - batch * p.q_len) * p.q_stride_qpos;
+#pragma unroll 1
+  for (int n = tid >> 2; n < columns; n += 32) {
+    const uint4* src = reinterpret_cast<const uint4*>(q + int64_t(n < p.heads ? n : 0) * p.q_stride_head) + (tid & 3) * 9;
+    uint4 v[9];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) v[i] = __ldcg(src + i);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = hmax2_abs_nan(hmax2_abs_nan(top, e4m3x2_to_f16x2(w[j] & 0xffff)), e4m3x2_to_f16x2(w[j] >> 16));
+    }
+    if ((top & 0x7fff) > 0x7c00 || (top >> 16) > 0x7c00) {  // NaN among them: they count as zero
+      top = 0;
+#pragma unroll
+      for (int i = 0; i < 9; ++i) {
+        uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (((w[j] >> (8 * k)) & 0x7f) == 0x7f) w[j] &= ~(0xffu << (8 * k));
+          top = hmax2_abs_nan(hmax2_abs_nan(top, e4m3x2_to_f16x2(w[j] & 0xffff)), e4m3x2_to_f16x2(w[j] >> 16));
+        }
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    __syncwarp();
+    uint32_t most = max(top & 0xffff, top >> 16);  // (non-negative halves order as integers)
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = max(int(most >> 10) - 8, 1);  // exponent field of the E4M3 binade
+    const uint32_t half = uint32_t(15 + 13 - e) << 10, times = half | half << 16;  // 2^(13 - e)
+    if ((tid & 3) == 0) unit[n] = __uint_as_float(uint32_t(127 + e - 13) << 23);
+    char* dst = b_smem + (n >> 3) * 512 + (n & 7) * 64;
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t out[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        out[j] = __byte_perm(hfma2(e4m3x2_to_f16x2(w[j] & 0xffff), times, 0x66006600u), hfma2(e4m3x2_to_f16x2(w[j] >> 16), times, 0x66006600u), 0x6420);
+      const int chunk = (tid & 3) * 9 + i;
+      *reinterpret_cast<uint4*>(dst + (chunk >> 2) * (columns * 64) + (((chunk & 3) ^ ((n >> 1) & 3)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int row0, int rows, int columns) {
+  extern __shared__ char raw[];
+  char* a_smem = raw + ((1024 - (ptx::smem_u32(raw) & 1023)) & 1023);
+  char* b_smem = a_smem + kStages * kStageBytes;
+  Small& s = *reinterpret_cast<Small*>(b_smem + columns * kQDim);
+  const Ctx c{p, s};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      ptx::mbar_init(bar(s.full_a[i]), kLoadWarps);
+      ptx::mbar_init(bar(s.empty_a[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(bar(s.full_d[i]), 1);
+      ptx::mbar_init(bar(s.empty_d[i]), kEpiWarps);
+    }
+    ptx::mbar_init(bar(s.full_b), kEpiWarps);
+    ptx::mbar_init(bar(s.drained), 1);
+    s.abort = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(&s.tmem), kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int r = tid; r < rows; r += kThreads) {
+    const Seen v = seen(p, row0 + r);
+    s.candidates[r] = v.used > p.budget ? v.used - p.sink - p.local : 0;
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  if (warp == 0) {  // this CTA's share: tiles [T i / n, T (i + 1) / n) of all tiles in the order of the rows
+    long long total = 0;
+    for (int base = 0; base < rows; base += 32)
+      total += __reduce_add_sync(0xffffffffu, base + lane < rows ? (s.candidates[base + lane] + kPages - 1) / kPages : 0);
+    const long long lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+    long long at = 0;
+    for (int base = 0; base < rows && at <= lo && hi > lo; base += 32) {
+      const int mine = base + lane < rows ? (s.candidates[base + lane] + kPages - 1) / kPages : 0;
+      int sum = mine;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        sum += lane >= o ? up : 0;
+      }
+      if (at + sum > lo && at + sum - mine <= lo) {
+        s.first_row = base + lane;
+        s.first_tile = int(lo - (at + sum - mine));
+      }
+      at += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) s.tiles = int(hi - lo);
+  }
+  __syncthreads();
+
+  if (s.tiles > 0) {
+    if (warp >= kFirstLoad) {
+      // ------------------------------------------------------------------ loads
+      const int w = warp - kFirstLoad, in8 = lane >> 2, chunk = lane & 3;
+      const int32_t most = int32_t(p.num_pages);
+      Walk k(s);
+      auto page_of = [&](int half) {  // of this lane's row of a tile; 0 for one that nobody reads
+        const int i = k.tile * kPages + (2 * w + half) * 8 + in8;
+        int page = 0;
+        if (k.left > 0 && i < k.candidates[k.row]) page = __ldcg(p.block_tables + int64_t((row0 + k.row) / p.q_len) * p.block_table_stride + p.sink + i);
+        return page >= 0 && page < most ? page : 0;
+      };
+      int page[2] = {page_of(0), page_of(1)};
+      bool ok = true;
+      int n = 0;
+      for (; k.left > 0; ++n) {
+        const int st = n & 1;
+        if (n >= kStages) ok = wait(c, s.empty_a[st], ((n >> 1) - 1) & 1);
+        if (!ok) break;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int8_t* src = p.summary + int64_t(page[half]) * kQDim + chunk * 16;
+          const uint32_t dst = ptx::smem_u32(a_smem) + st * kStageBytes + (2 * w + half) * 512 + in8 * 64 + ((chunk ^ ((in8 >> 1) & 3)) << 4);
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) cp_async16(dst + b * (kPages * 64), src + b * 64);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        k.next();
+        page[0] = page_of(0);
+        page[1] = page_of(1);
+        if (n > 0) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(s.full_a[st ^ 1]));
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (ok && lane == 0) ptx::mbar_arrive(bar(s.full_a[(n - 1) & 1]));
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------------ MMAs
+      const uint32_t e = ptx::elect_one();
+      const uint64_t a0 = ptx::smem_desc(ptx::smem_u32(a_smem), 16, 512, 4), b0 = ptx::smem_desc(ptx::smem_u32(b_smem), 16, 512, 4);
+      // D: S32; A, B: signed 8-bit, K-major
+      const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(columns >> 3) << 17) | (uint32_t(kPages >> 4) << 24);
+      int seg = 0;
+      bool fresh = true, ok = true;
+      Walk k(s);
+      for (int n = 0; k.left > 0 && ok; ++n) {
+        const int st = n & 1;
+        if (fresh) ok = wait(c, s.full_b, seg & 1);
+        if (ok && n >= 2) ok = wait(c, s.empty_d[st], ((n >> 1) - 1) & 1);
+        if (ok) ok = wait(c, s.full_a[st], (n >> 1) & 1);
+        if (!ok) break;
+        ptx::tc_fence_after();
+#pragma unroll
+        for (uint32_t i = 0; i < kQDim / 32; ++i)
+          ptx::umma_i8(e, tmem + st * 128, a0 + ((st * kStageBytes + (i >> 1) * (kPages * 64)) >> 4) + 2 * (i & 1),
+                       b0 + (((i >> 1) * (columns * 64)) >> 4) + 2 * (i & 1), idesc, i);
+        if (e) ptx::umma_commit(bar(s.empty_a[st]));
+        if (e) ptx::umma_commit(bar(s.full_d[st]));
+        fresh = k.row_ends();
+        seg += fresh;
+        k.next();
+      }
+      // nothing is in flight when TMEM is given back; the MMAs wait for nobody, so this ends whatever the poll budget is
+      if (e) ptx::umma_commit(bar(s.drained));
+      for (uint32_t i = 0; i < max(p.wait_polls, 1u << 16) && !ptx::mbar_try_wait(bar(s.drained), 0); ++i) {
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------------------------ the query's integers, and scores
+      Walk k(s);
+      int seg = 0;
+      make_b(p, b_smem, s.unit[0], row0 + k.row, columns);
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(s.full_b));
+      ptx::bar_sync(1, 32 * kEpiWarps);
+      for (int n = 0; k.left > 0; ++n) {
+        const int st = n & 1, i = k.tile * kPages + tid;
+        int page = -1;
+        float scale = 0.f;
+        if (i < k.candidates[k.row]) {
+          page = __ldcg(p.block_tables + int64_t((row0 + k.row) / p.q_len) * p.block_table_stride + p.sink + i);
+          if (page >= p.num_pages) page = -1;
+          if (page >= 0) scale = __ldcg(p.summary_sf + page);
+        }
+        const bool ok = wait(c, s.full_d[st], (n >> 1) & 1);
+        // Units and codes of the next row are all there, and those of the row before no longer read, behind the barrier at the end; a warp
+        // that gave up takes the others along.
+        if (!ok) {
+          ptx::bar_or(1, 32 * kEpiWarps, true);
+          break;
+        }
+        const float* unit = s.unit[seg & 1];
+        if (k.row_ends() && k.left > 1) {  // the MMAs of this row are over: the next row's query takes the place of its own
+          ++seg;
+          make_b(p, b_smem, s.unit[seg & 1], row0 + k.next_row(), columns);
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(s.full_b));
+        }
+        ptx::tc_fence_after();
+        float best = __uint_as_float(0xff800000u);
+#pragma unroll 1
+        for (int col = 0; col < columns; col += 16) {
+          uint32_t d[16];
+          ptx::tmem_ld16(tmem + (uint32_t(warp) << 21) + st * 128 + col, d);
+          float u[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(u + 4 * j) = *reinterpret_cast<const float4*>(unit + col + 4 * j);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) best = fmaxf(best, float(int(d[j])) * u[j]);
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(s.empty_d[st]));
+        if (i < k.candidates[k.row]) p.keys[int64_t(row0 + k.row) * p.width + i] = page >= 0 ? key_of(best * scale) : 0u;
+        if (ptx::bar_or(1, 32 * kEpiWarps, false)) break;
+        k.next();
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+size_t smem_bytes(int columns) { return 1024 + size_t(kStages) * kStageBytes + size_t(columns) * kQDim + sizeof(Small); }
+static_assert(1024 + kStages * kStageBytes + 128 * kQDim + sizeof(Small) <= 232448, "shared memory of a CTA");
+
+}  // namespace
+
+cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream) {
+  const int rows = p.batch * p.q_len, columns = (p.heads + 15) / 16 * 16;
+  const size_t smem = smem_bytes(columns);
+  cudaError_t e = cudaFuncSetAttribute(score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_bytes(128)));
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (p.width - p.sink - p.local + kPages - 1) / kPages;  // of the longest row that the tables can hold
+  for (int row0 = 0; row0 < rows; row0 += kMaxRows) {
+    const int n = rows - row0 < kMaxRows ? rows - row0 : kMaxRows;
+    const int64_t most = tiles * n;
+    e = launch_dependent(score_kernel, dim3(unsigned(most < sms ? most : sms)), kThreads, smem, stream, p, row0, n, columns);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace mla

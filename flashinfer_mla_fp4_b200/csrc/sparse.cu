@@ -10,20 +10,14 @@
 // Score of a page for a query: the query's heads as integers q_h = round(q 2^k_h), k_h bringing the head's largest binade to
 // [64, 128) (E4M3 values of the three largest binades are exact), dots <q_h, code> in int32 (below 2^24), and
 // scale * max_h 2^-k_h <q_h, code> with one rounding at the end.  So scores too are the same wherever they are made, and pages that
-// tie do so by value.
+// tie do so by value.  The scores are made in score_sm100.cu.
 #include <math_constants.h>
 
-#include "common.cuh"
-#include "launch.h"
+#include "sparse.cuh"
 
 namespace mla {
 
 namespace {
-
-__device__ __forceinline__ void dependent_launch() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
 
 // ------------------------------------------------------------------------------------------ summaries
 constexpr int kSumThreads = 320;  // 256: latent, four groups of tokens x 64 words of a row; 64: RoPE, four groups x 16 words
@@ -118,89 +112,6 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
   if (tid == 0) p.summary_sf[page] = sound ? scale : CUDART_NAN_F;
 }
 
-// ------------------------------------------------------------------------------------------ scores
-constexpr int kScoreThreads = 256;
-constexpr int kScorePages = 64;             // pages per CTA
-constexpr int kWordsQ = kQDim / 4;          // 144 words of four codes
-constexpr int kPadWords = kWordsQ + 1;      // a head's row in shared memory, padded against bank conflicts
-
-// What a query position sees of its request.
-struct Seen {
-  int len, used;  // tokens, pages
-};
-__device__ __forceinline__ Seen seen(const SelectParams& p, int row) {
-  const int b = row / p.q_len, i = row - b * p.q_len;
-  int len = min(p.seq_lens[b], p.seq_cap);
-  if (p.causal) len -= p.q_len - 1 - i;
-  len = max(len, 0);
-  return {len, (len - 1 + p.page_size) / p.page_size};
-}
-// a score as an integer that orders as the score does: NaN first, then by value, zeros of either sign alike
-__device__ __forceinline__ uint32_t key_of(float score) {
-  if (score != score) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(score + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(SelectParams p) {
-  extern __shared__ uint32_t q_s[];  // [heads][kPadWords] codes, then [heads] units, then [8 warps][kWordsQ] a page each
-  dependent_launch();
-  const int row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Seen v = seen(p, row);
-  if (v.used <= p.budget) return;
-  const int candidates = v.used - p.sink - p.local, first = blockIdx.x * kScorePages;
-  if (first >= candidates) return;
-  float* unit_s = reinterpret_cast<float*>(q_s + p.heads * kPadWords);
-  uint32_t* page_s = q_s + p.heads * (kPadWords + 1) + warp * kWordsQ;
-  const int b = row / p.q_len, i = row - b * p.q_len;
-  const uint8_t* q = p.q + b * p.q_stride_batch + i * p.q_stride_qpos;
-  for (int h = warp; h < p.heads; h += kScoreThreads / 32) {
-    const uint32_t* qh = reinterpret_cast<const uint32_t*>(q + h * p.q_stride_head);
-    uint32_t w[5], e = 1;
-    for (int k = 0; k < 5; ++k) {
-      w[k] = lane + 32 * k < kWordsQ ? qh[lane + 32 * k] : 0;
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t m = (w[k] >> (8 * j)) & 0x7f;
-        if (m != 0x7f) e = max(e, m >> 3);
-      }
-    }
-    e = __reduce_max_sync(0xffffffffu, e);
-    for (int k = 0; k < 5; ++k) {
-      if (lane + 32 * k >= kWordsQ) break;
-      uint32_t out = 0;
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t byte = (w[k] >> (8 * j)) & 0xff;
-        // value * 2^(13 - e), from 512 times the value
-        const float x = (byte & 0x7f) == 0x7f ? 0.f : float(e4m3_512(byte)) * __uint_as_float((127 + 4 - e) << 23);
-        out |= (uint32_t(__float2int_rn(x)) & 0xff) << (8 * j);
-      }
-      q_s[h * kPadWords + lane + 32 * k] = out;
-    }
-    if (lane == 0) unit_s[h] = __uint_as_float((127 + e - 13) << 23);
-  }
-  __syncthreads();
-  const int32_t* table = p.block_tables + int64_t(b) * p.block_table_stride + p.sink;
-  for (int c = first + warp; c < min(first + kScorePages, candidates); c += kScoreThreads / 32) {
-    const int page = table[c];
-    uint32_t key = 0;  // a page outside the pool comes last
-    if (page >= 0 && page < p.num_pages) {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.summary + int64_t(page) * kQDim);
-      __syncwarp();
-      for (int k = lane; k < kWordsQ; k += 32) page_s[k] = src[k];
-      __syncwarp();
-      float best = -CUDART_INF_F;
-      for (int h = lane; h < p.heads; h += 32) {
-        int dot = 0;
-        for (int k = 0; k < kWordsQ; ++k) dot = __dp4a(int(q_s[h * kPadWords + k]), int(page_s[k]), dot);
-        best = fmaxf(best, float(dot) * unit_s[h]);
-      }
-      for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-      key = key_of(best * p.summary_sf[page]);
-    }
-    if (lane == 0) p.keys[int64_t(row) * p.width + c] = key;
-  }
-}
-
 // ------------------------------------------------------------------------------------------ selection
 constexpr int kSelThreads = 512;
 
@@ -246,7 +157,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(SelectParams p) {
     for (int k = tid; k < 256; k += kSelThreads) hist_s[k] = 0;
     __syncthreads();
     for (int k = tid; k < candidates; k += kSelThreads)
-      if (shift == 24 || (keys[k] >> (shift + 8)) == prefix) atomicAdd(&hist_s[(keys[k] >> shift) & 255], 1);
+      if (shift == 24 || (__ldcg(keys + k) >> (shift + 8)) == prefix) atomicAdd(&hist_s[(__ldcg(keys + k) >> shift) & 255], 1);
     __syncthreads();
     if (tid == 0) {
       uint32_t above = 0;
@@ -262,7 +173,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(SelectParams p) {
   int taken = 0, ties = 0;
   for (int base = 0; base < candidates; base += kSelThreads) {
     const int k = base + tid;
-    const uint32_t key = k < candidates ? keys[k] : 0;
+    const uint32_t key = k < candidates ? __ldcg(keys + k) : 0;
     int n, m;
     const bool tie = k < candidates && key == prefix;
     const int before = scan_before(tie, warp_s, &n);
@@ -274,37 +185,18 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(SelectParams p) {
   }
 }
 
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 }  // namespace
 
 cudaError_t launch_summarize(const SummarizeParams& p, int64_t ctas, cudaStream_t stream) {
   return launch_dependent(summarize_kernel, dim3(unsigned(ctas)), kSumThreads, 0, stream, p);
 }
 
-cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
-  const int rows = p.batch * p.q_len, most = p.width - p.sink - p.local;  // candidates of the longest request
+cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream) {
   if (p.width > p.budget) {
-    const size_t smem = size_t(p.heads) * (kPadWords + 1) * 4 + size_t(kScoreThreads / 32) * kWordsQ * 4;
-    cudaError_t e = cudaFuncSetAttribute(score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
-    e = launch_dependent(score_kernel, dim3(unsigned((most + kScorePages - 1) / kScorePages), unsigned(rows)), kScoreThreads, smem, stream, p);
+    cudaError_t e = launch_score(p, sms, stream);
     if (e != cudaSuccess) return e;
   }
-  return launch_dependent(select_kernel, dim3(unsigned(rows)), kSelThreads, 0, stream, p);
+  return launch_dependent(select_kernel, dim3(unsigned(p.batch * p.q_len)), kSelThreads, 0, stream, p);
 }
 
 }  // namespace mla

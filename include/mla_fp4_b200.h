@@ -318,7 +318,8 @@ typedef struct MlaFp4SelectArgs {
   int32_t width;           /* pages per block-table row; lengths beyond width * page_size are cut to it */
   int32_t budget, sink_pages, local_pages;
   int32_t causal;
-  int32_t reserved;        /* 0 */
+  int32_t wait_polls;      /* as in MlaFp4DecodeArgs; after a wait that ran out the selection is of valid pages, but not the best */
+  int32_t* status;         /* as in MlaFp4DecodeArgs; may be NULL */
   void* stream;
 } MlaFp4SelectArgs;
 int mla_fp4_select_workspace_bytes(int32_t batch, int32_t q_len, int32_t width, size_t* bytes_out);
