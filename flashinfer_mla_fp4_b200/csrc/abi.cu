@@ -480,6 +480,8 @@ int summarize(mla::SummarizeParams& p, int64_t ctas, void* stream) {
   if (e != cudaSuccess) return fail(MLA_FP4_ERR_CUDA, std::string("summarize launch: ") + cudaGetErrorString(e));
   return MLA_FP4_OK;
 }
+// scores of a row in the workspace: rows start on 16 bytes
+size_t select_key_stride(int width) { return (size_t(width) + 3) / 4 * 4; }
 // the most tokens of a request, with room for arithmetic on them
 int table_cap(int width, int page_size) { return std::min(seq_cap_of(width, page_size), INT_MAX - 256); }
 }  // namespace
@@ -516,7 +518,7 @@ int mla_fp4_summarize_new_pages(const void* kv_cache, const float* kv_cache_sf, 
 
 int mla_fp4_select_workspace_bytes(int32_t batch, int32_t q_len, int32_t width, size_t* bytes_out) {
   if (!bytes_out || batch < 0 || q_len <= 0 || width < 0) return fail(MLA_FP4_ERR_BAD_ARG, "batch/q_len/width out of range");
-  *bytes_out = size_t(batch) * size_t(q_len) * size_t(width) * 4;
+  *bytes_out = size_t(batch) * size_t(q_len) * select_key_stride(width) * 4;
   return MLA_FP4_OK;
 }
 
@@ -551,6 +553,7 @@ int mla_fp4_select_pages(const MlaFp4SelectArgs* a) {
   p.block_tables = a->block_tables; p.seq_lens = a->seq_lens;
   p.selected = a->selected; p.selected_lens = a->selected_lens;
   p.keys = static_cast<uint32_t*>(a->workspace);
+  p.key_stride = int64_t(select_key_stride(a->width));
   p.block_table_stride = a->block_table_stride; p.num_pages = a->num_pages;
   p.batch = a->batch; p.q_len = a->q_len; p.heads = a->num_heads; p.page_size = a->page_size; p.width = a->width;
   p.budget = a->budget; p.sink = a->sink_pages; p.local = a->local_pages; p.causal = a->causal ? 1 : 0;

@@ -121,7 +121,8 @@ struct SelectParams {
   const int32_t* seq_lens;
   int32_t* selected;       // [rows][budget]
   int32_t* selected_lens;  // [rows]
-  uint32_t* keys;          // workspace: [rows][width]
+  uint32_t* keys;          // workspace: [rows][key_stride]
+  int64_t key_stride;
   int64_t block_table_stride, num_pages;
   int32_t batch, q_len, heads, page_size, width, budget, sink, local, causal;
   int32_t seq_cap;  // as in DecodeParams

@@ -9,8 +9,9 @@
 // 64-byte swizzle of the operand (576 = 9 x 64 without a rest; eight rows x 64 bytes per instruction are one swizzle atom: no bank
 // conflicts, whole sectors); a TMA gather would take 288 instructions of 256 bytes a tile.
 //
-// Roles: warps 0-3 turn a row's query into integers (the B operand) and take the scores out of TMEM, warp 4 issues the MMAs, warps
-// 5-12 load.  All waits are bounded; one that runs out sets the status and ends the CTA, whose keys are then not all written.
+// Roles: warps 0-3 take the scores out of TMEM, warp 4 issues the MMAs, warps 5-12 load, and turn a row's query into integers (the B
+// operand) while the row's first two tiles are on their way.  All waits are bounded; one that runs out sets the status and ends the CTA, whose
+// keys are then not all written.
 #include "common.cuh"
 #include "launch.h"
 #include "ptx_sm100.cuh"
@@ -24,7 +25,8 @@ constexpr int kEpiWarps = 4, kLoadWarps = 8;
 constexpr int kMmaWarp = kEpiWarps, kFirstLoad = kEpiWarps + 1;
 constexpr int kThreads = 32 * (kEpiWarps + 1 + kLoadWarps);
 constexpr int kPages = 128;                       // pages of a tile: the lanes of TMEM
-constexpr int kBlocks = kQDim / 64;               // 64-byte blocks of a summary
+constexpr int kBlocks = kQDim / 64;               // 64-byte blocks of a row: of the operands' swizzle
+constexpr int kChunks = kQDim / 16;               // 16-byte chunks
 constexpr int kStageBytes = kPages * kQDim;       // [9 blocks][128 pages][64 bytes], 64-byte swizzle
 constexpr int kStages = 2;
 constexpr int kMaxRows = 1024;                    // rows of a launch (the launcher makes several)
@@ -33,7 +35,7 @@ constexpr uint32_t kTmemCols = 256;               // two accumulators of up to 1
 // shared memory, from a 1024-byte boundary on: the stages, the query's codes [9][columns][64 bytes], then
 struct Small {
   int candidates[kMaxRows];  // pages that a row scores
-  float unit[2][128];        // 2^-k of the heads, of the row in hand and the one before
+  float unit[4][128];        // 2^-k of the heads, by row: an epilogue may be three tiles, so three rows, behind the loads
   unsigned long long full_a[kStages], empty_a[kStages], full_d[2], empty_d[2], full_b, drained;
   uint32_t tmem;
   int first_row, first_tile, tiles;  // of this CTA
@@ -79,6 +81,11 @@ struct Walk {
     if (!row_ends()) ++tile;
     else if (left > 0) row = next_row(), tile = 0;
   }
+  // block-table entry of page i of the tile, -1 where there is none
+  __device__ __forceinline__ int entry(const SelectParams& p, int row0, int i) const {
+    i += tile * kPages;
+    return left > 0 && i < candidates[row] ? __ldcg(p.block_tables + int64_t((row0 + row) / p.q_len) * p.block_table_stride + p.sink + i) : -1;
+  }
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -90,68 +97,91 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
   asm("{\n\t.reg .b16 b;\n\tcvt.u16.u32 b, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(two_bytes));
   return r;
 }
-__device__ __forceinline__ uint32_t hmax2_abs_nan(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("{\n\t.reg .b32 t;\n\tand.b32 t, %2, 0x7fff7fff;\n\tmax.NaN.f16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
 
-// The heads of a row's query as integers, into shared memory: by the 128 threads of the epilogue, four lanes a head, 144 values each.  In FP16: an
-// E4M3 value times 2^k is exact, and adding 1536 rounds it to a whole number (to even, as round() does) that is the low byte of the sum.
-// Columns behind the last head repeat head 0, which leaves the largest score as it is.
-__device__ __forceinline__ void make_b(const SelectParams& p, char* b_smem, float* unit, int row, int columns) {
-  const int batch = row / p.q_len, tid = threadIdx.x;
+// The 16-byte chunks of a warp's `rows` consecutive rows of 576 bytes, 32 at a time in the order of their addresses: f(row, chunk of it).
+struct Chunks {
+  int row = 0, chunk = threadIdx.x & 31;
+  __device__ __forceinline__ void next() {
+    chunk += 32;
+    const bool over = chunk >= kChunks;
+    chunk -= over ? kChunks : 0;
+    row += over;
+  }
+};
+template <typename F>
+__device__ __forceinline__ void for_chunks(int rows, F f) {
+#pragma unroll 3
+  for (Chunks c; c.row < rows; c.next()) f(c.row, c.chunk);
+}
+// where a chunk of a row lies in an operand of `rows` rows: [9 blocks][rows][64 bytes], 64-byte swizzle
+__device__ __forceinline__ uint32_t operand_at(int rows, int row, int chunk) {
+  return uint32_t((chunk >> 2) * (rows * 64) + row * 64 + (((chunk & 3) ^ ((row >> 1) & 3)) << 4));
+}
+
+// The heads of a row's query, to be the B operand: first fetched as they are, ...  Columns behind the last head repeat head 0, which leaves the
+// largest score as it is.
+__device__ __forceinline__ void fetch_b(const SelectParams& p, uint32_t b_smem, int row, int columns) {
+  const int each = columns / kLoadWarps, first = ((threadIdx.x >> 5) - kFirstLoad) * each, batch = row / p.q_len;
   const uint8_t* q = p.q + batch * p.q_stride_batch + (row - batch * p.q_len) * p.q_stride_qpos;
+  for_chunks(each, [&](int r, int chunk) {
+    const int head = first + r;
+    cp_async16(b_smem + operand_at(columns, head, chunk), q + int64_t(head < p.heads ? head : 0) * p.q_stride_head + 16 * chunk);
+  });
+}
+// ... then turned into integers where they lie: four lanes a head, eight heads at a time (a swizzle atom per access: no bank conflicts).  In FP16: an
+// E4M3 value times 2^k is exact, and adding 1536 rounds it to a whole number (to even, as round() does) that is the low byte of the sum.
+__device__ __forceinline__ void convert_b(char* b_smem, float* unit, int columns) {
+  const int each = columns / kLoadWarps, first = ((threadIdx.x >> 5) - kFirstLoad) * each, lane = threadIdx.x & 31;
 #pragma unroll 1
-  for (int n = tid >> 2; n < columns; n += 32) {
-    const uint4* src = reinterpret_cast<const uint4*>(q + int64_t(n < p.heads ? n : 0) * p.q_stride_head) + (tid & 3) * 9;
-    uint4 v[9];
-#pragma unroll
-    for (int i = 0; i < 9; ++i) v[i] = __ldcg(src + i);
+  for (int r = lane >> 2; r < (each + 7) / 8 * 8; r += 8) {
+    const int head = first + (r < each ? r : 0);
+    uint4 v[kBlocks];
+    // the largest magnitude: bytes without their signs, by 16 bits; NaN is 127
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 9; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int i = 0; i < kBlocks; ++i) v[i] = *reinterpret_cast<const uint4*>(b_smem + operand_at(columns, head, 4 * i + (lane & 3)));
+    auto top_of = [](const uint4& x) {
+      const uint32_t a = __vmaxu2(x.x & 0x7f007f, x.y & 0x7f007f), b = __vmaxu2(x.z & 0x7f007f, x.w & 0x7f007f);
+      const uint32_t c = __vmaxu2((x.x >> 8) & 0x7f007f, (x.y >> 8) & 0x7f007f), d = __vmaxu2((x.z >> 8) & 0x7f007f, (x.w >> 8) & 0x7f007f);
+      return __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d));
+    };
 #pragma unroll
-      for (int j = 0; j < 4; ++j) top = hmax2_abs_nan(hmax2_abs_nan(top, e4m3x2_to_f16x2(w[j] & 0xffff)), e4m3x2_to_f16x2(w[j] >> 16));
-    }
-    if ((top & 0x7fff) > 0x7c00 || (top >> 16) > 0x7c00) {  // NaN among them: they count as zero
+    for (int i = 0; i < kBlocks; ++i) top = __vmaxu2(top, top_of(v[i]));
+    if ((top & 0xffff) == 0x7f || top >> 16 == 0x7f) {  // NaN among them: they count as zero
       top = 0;
 #pragma unroll
-      for (int i = 0; i < 9; ++i) {
-        uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      for (int i = 0; i < kBlocks; ++i) {
+        uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (((w[j] >> (8 * k)) & 0x7f) == 0x7f) w[j] &= ~(0xffu << (8 * k));
-          top = hmax2_abs_nan(hmax2_abs_nan(top, e4m3x2_to_f16x2(w[j] & 0xffff)), e4m3x2_to_f16x2(w[j] >> 16));
+          const uint32_t nan = ((x[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // the top bit of a byte that is NaN
+          x[j] &= ~(nan | (nan - (nan >> 7)));
         }
-        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        v[i] = make_uint4(x[0], x[1], x[2], x[3]);
+        top = __vmaxu2(top, top_of(v[i]));
       }
     }
     __syncwarp();
-    uint32_t most = max(top & 0xffff, top >> 16);  // (non-negative halves order as integers)
+    uint32_t most = max(top & 0xffff, top >> 16);
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int e = max(int(most >> 10) - 8, 1);  // exponent field of the E4M3 binade
-    const uint32_t half = uint32_t(15 + 13 - e) << 10, times = half | half << 16;  // 2^(13 - e)
-    if ((tid & 3) == 0) unit[n] = __uint_as_float(uint32_t(127 + e - 13) << 23);
-    char* dst = b_smem + (n >> 3) * 512 + (n & 7) * 64;
+    const int binade = max(int(most >> 3), 1);  // exponent field
+    const uint32_t half = uint32_t(15 + 13 - binade) << 10, times = half | half << 16;  // 2^(13 - binade)
+    if (r >= each) continue;
+    if ((lane & 3) == 0) unit[head] = __uint_as_float(uint32_t(127 + binade - 13) << 23);
 #pragma unroll
-    for (int i = 0; i < 9; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int i = 0; i < kBlocks; ++i) {
+      const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
       uint32_t out[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        out[j] = __byte_perm(hfma2(e4m3x2_to_f16x2(w[j] & 0xffff), times, 0x66006600u), hfma2(e4m3x2_to_f16x2(w[j] >> 16), times, 0x66006600u), 0x6420);
-      const int chunk = (tid & 3) * 9 + i;
-      *reinterpret_cast<uint4*>(dst + (chunk >> 2) * (columns * 64) + (((chunk & 3) ^ ((n >> 1) & 3)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+        out[j] = __byte_perm(hfma2(e4m3x2_to_f16x2(x[j] & 0xffff), times, 0x66006600u), hfma2(e4m3x2_to_f16x2(x[j] >> 16), times, 0x66006600u), 0x6420);
+      *reinterpret_cast<uint4*>(b_smem + operand_at(columns, head, 4 * i + (lane & 3))) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
 }
@@ -169,10 +199,10 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       ptx::mbar_init(bar(s.empty_a[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(bar(s.full_d[i]), 1);
+      ptx::mbar_init(bar(s.full_d[i]), 2);
       ptx::mbar_init(bar(s.empty_d[i]), kEpiWarps);
     }
-    ptx::mbar_init(bar(s.full_b), kEpiWarps);
+    ptx::mbar_init(bar(s.full_b), kLoadWarps);
     ptx::mbar_init(bar(s.drained), 1);
     s.abort = 0;
     ptx::fence_barrier_init();
@@ -217,44 +247,56 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
   if (s.tiles > 0) {
     if (warp >= kFirstLoad) {
       // ------------------------------------------------------------------ loads
-      const int w = warp - kFirstLoad, in8 = lane >> 2, chunk = lane & 3;
-      const int32_t most = int32_t(p.num_pages);
+      constexpr int kMine = kPages / kLoadWarps;  // a warp's pages of a tile
+      const int first = (warp - kFirstLoad) * kMine;
+      const uint32_t a_addr = ptx::smem_u32(a_smem), b_addr = ptx::smem_u32(b_smem);
       Walk k(s);
-      auto page_of = [&](int half) {  // of this lane's row of a tile; 0 for one that nobody reads
-        const int i = k.tile * kPages + (2 * w + half) * 8 + in8;
-        int page = 0;
-        if (k.left > 0 && i < k.candidates[k.row]) page = __ldcg(p.block_tables + int64_t((row0 + k.row) / p.q_len) * p.block_table_stride + p.sink + i);
-        return page >= 0 && page < most ? page : 0;
-      };
-      int page[2] = {page_of(0), page_of(1)};
+      // A row's query is fetched once the MMAs of the row before are over, which is known where the tile behind its first one is loaded.
+      fetch_b(p, b_addr, row0 + k.row, columns);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      // Page numbers come a tile ahead of their use, asked for before the rows of the tile before: behind those they would take as long.
+      int next_page = lane < kMine ? k.entry(p, row0, first + lane) : -1;
+      int fresh = -1, seg = 0;  // fresh: the row that the last tile was the first of, or -1
       bool ok = true;
-      int n = 0;
-      for (; k.left > 0; ++n) {
+      for (int n = 0; ; ++n) {
         const int st = n & 1;
         if (n >= kStages) ok = wait(c, s.empty_a[st], ((n >> 1) - 1) & 1);
         if (!ok) break;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int8_t* src = p.summary + int64_t(page[half]) * kQDim + chunk * 16;
-          const uint32_t dst = ptx::smem_u32(a_smem) + st * kStageBytes + (2 * w + half) * 512 + in8 * 64 + ((chunk ^ ((in8 >> 1) & 3)) << 4);
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) cp_async16(dst + b * (kPages * 64), src + b * 64);
+        if (fresh >= 0 && seg > 0) {
+          fetch_b(p, b_addr, row0 + fresh, columns);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        const bool more = k.left > 0;
+        const int next_fresh = more && (n == 0 || k.tile == 0) ? k.row : -1;
+        if (more) {
+          k.next();
+          const int page = next_page >= 0 && next_page < p.num_pages ? next_page : 0;  // (0 for one that nobody reads)
+          next_page = lane < kMine ? k.entry(p, row0, first + lane) : -1;
+          for_chunks(kMine, [&](int r, int chunk) {
+            const int from = __shfl_sync(0xffffffffu, page, r);
+            cp_async16(a_addr + st * kStageBytes + operand_at(kPages, first + r, chunk), p.summary + int64_t(from) * kQDim + 16 * chunk);
+          });
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        k.next();
-        page[0] = page_of(0);
-        page[1] = page_of(1);
         if (n > 0) {
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          if (fresh >= 0) {
+            if (seg == 0) asm volatile("cp.async.wait_group 2;" ::: "memory");  // the query came first, both tiles may still be on their way
+            else asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();  // (a lane converts what others have fetched)
+            convert_b(b_smem, s.unit[seg++ & 3], columns);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(s.full_b));
+          }
+          asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the tile just asked for
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(bar(s.full_a[st ^ 1]));
         }
+        fresh = next_fresh;
+        if (!more) break;
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (ok && lane == 0) ptx::mbar_arrive(bar(s.full_a[(n - 1) & 1]));
     } else if (warp == kMmaWarp) {
       // ------------------------------------------------------------------ MMAs
       const uint32_t e = ptx::elect_one();
@@ -276,7 +318,10 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
           ptx::umma_i8(e, tmem + st * 128, a0 + ((st * kStageBytes + (i >> 1) * (kPages * 64)) >> 4) + 2 * (i & 1),
                        b0 + (((i >> 1) * (columns * 64)) >> 4) + 2 * (i & 1), idesc, i);
         if (e) ptx::umma_commit(bar(s.empty_a[st]));
-        if (e) ptx::umma_commit(bar(s.full_d[st]));
+        if (e) {
+          ptx::umma_commit(bar(s.full_d[st]));
+          ptx::mbar_arrive(bar(s.full_d[st]));  // (hands on what the load warps have written for the epilogue: the units)
+        }
         fresh = k.row_ends();
         seg += fresh;
         k.next();
@@ -287,38 +332,17 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       }
       __syncwarp();
     } else {
-      // ------------------------------------------------------------------ the query's integers, and scores
+      // ------------------------------------------------------------------ scores
       Walk k(s);
-      int seg = 0;
-      make_b(p, b_smem, s.unit[0], row0 + k.row, columns);
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar(s.full_b));
-      ptx::bar_sync(1, 32 * kEpiWarps);
+      int seg = 0, next_page = k.entry(p, row0, tid);
       for (int n = 0; k.left > 0; ++n) {
-        const int st = n & 1, i = k.tile * kPages + tid;
-        int page = -1;
-        float scale = 0.f;
-        if (i < k.candidates[k.row]) {
-          page = __ldcg(p.block_tables + int64_t((row0 + k.row) / p.q_len) * p.block_table_stride + p.sink + i);
-          if (page >= p.num_pages) page = -1;
-          if (page >= 0) scale = __ldcg(p.summary_sf + page);
-        }
-        const bool ok = wait(c, s.full_d[st], (n >> 1) & 1);
-        // Units and codes of the next row are all there, and those of the row before no longer read, behind the barrier at the end; a warp
-        // that gave up takes the others along.
-        if (!ok) {
-          ptx::bar_or(1, 32 * kEpiWarps, true);
-          break;
-        }
-        const float* unit = s.unit[seg & 1];
-        if (k.row_ends() && k.left > 1) {  // the MMAs of this row are over: the next row's query takes the place of its own
-          ++seg;
-          make_b(p, b_smem, s.unit[seg & 1], row0 + k.next_row(), columns);
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(s.full_b));
-        }
+        const int st = n & 1, row = k.row, i = k.tile * kPages + tid, page = next_page;
+        const bool mine = i < k.candidates[row], last = k.row_ends(), there = page >= 0 && page < p.num_pages;
+        const float scale = there ? __ldcg(p.summary_sf + page) : 0.f;
+        k.next();
+        next_page = k.entry(p, row0, tid);
+        if (!wait(c, s.full_d[st], (n >> 1) & 1)) break;
+        const float* unit = s.unit[seg & 3];
         ptx::tc_fence_after();
         float best = __uint_as_float(0xff800000u);
 #pragma unroll 1
@@ -335,9 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(s.empty_d[st]));
-        if (i < k.candidates[k.row]) p.keys[int64_t(row0 + k.row) * p.width + i] = page >= 0 ? key_of(best * scale) : 0u;
-        if (ptx::bar_or(1, 32 * kEpiWarps, false)) break;
-        k.next();
+        if (mine) p.keys[int64_t(row0 + row) * p.key_stride + i] = there ? key_of(best * scale) : 0u;
+        seg += last;
       }
     }
   }

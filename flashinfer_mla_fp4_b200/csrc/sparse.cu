@@ -113,76 +113,119 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
 }
 
 // ------------------------------------------------------------------------------------------ selection
-constexpr int kSelThreads = 512;
+// A CTA per row.  A thread has kKeys consecutive keys in registers; the key of the last page that is taken is found by halving the range of the
+// keys until as many lie above the middle as are wanted, which takes about log2(candidates) + 2 counts, 32 where pages tie: a count is a
+// compare per key, a reduction in the warp and one across warps behind one barrier.  (By bytes through a histogram in shared memory, whose
+// counters of the leading byte everybody wants, 2045 of 64 rows took 39 us.)  Then one scan gives each page that is taken its place.
+// kKeys = 0: more candidates than registers hold; the keys stay in global memory, read through L2 at each count.
+constexpr int kSelMost = 1024;
 
-// Sum over the CTA of the values before this thread's; *total: of all.
-__device__ __forceinline__ int scan_before(bool flag, int* warp_s, int* total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ballot = __ballot_sync(0xffffffffu, flag);
-  __syncthreads();
-  if (lane == 0) warp_s[warp] = __popc(ballot);
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kSelThreads / 32; ++w) {
-    const int n = warp_s[w];
-    before += w < warp ? n : 0;
-    all += n;
-  }
-  *total = all;
-  return before + __popc(ballot & ((1u << lane) - 1));
-}
-
-__global__ void __launch_bounds__(kSelThreads) select_kernel(SelectParams p) {
-  __shared__ int hist_s[256], warp_s[kSelThreads / 32];
-  __shared__ uint32_t digit_s, above_s;
+template <int kKeys>
+__global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
+  __shared__ uint32_t sum_s[2][32], range_s[2][32];
   dependent_launch();
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+  const uint32_t* keys = p.keys + int64_t(row) * p.key_stride;
   const Seen v = seen(p, row);
   const int32_t* table = p.block_tables + int64_t(row / p.q_len) * p.block_table_stride;
   int32_t* out = p.selected + int64_t(row) * p.budget;
   if (v.used <= p.budget) {  // the budget holds them all
-    for (int k = tid; k < p.budget; k += kSelThreads) out[k] = k < v.used ? table[k] : 0;
+    for (int k = tid; k < p.budget; k += blockDim.x) out[k] = k < v.used ? __ldcg(table + k) : 0;
     if (tid == 0) p.selected_lens[row] = v.len;
     return;
   }
   const int candidates = v.used - p.sink - p.local, wanted = p.budget - p.sink - p.local;
-  const uint32_t* keys = p.keys + int64_t(row) * p.width;
-  for (int k = tid; k < p.sink; k += kSelThreads) out[k] = table[k];
-  for (int k = tid; k < p.local; k += kSelThreads) out[p.budget - p.local + k] = table[v.used - p.local + k];
+  const int mine = kKeys ? kKeys : (candidates + int(blockDim.x) - 1) / int(blockDim.x);
+  const int first = tid * mine, last = min(first + mine, candidates);
+  uint32_t reg[kKeys ? kKeys : 1];
+  if constexpr (kKeys > 0) {
+#pragma unroll
+    for (int i = 0; i < kKeys; i += 4) {  // (a row has room for whole groups of four; what lies behind the candidates is not looked at)
+      if (first + i >= candidates) break;
+      const uint4 four = __ldcg(reinterpret_cast<const uint4*>(keys + first + i));
+      reg[i] = four.x;
+      reg[i + 1] = four.y;
+      reg[i + 2] = four.z;
+      reg[i + 3] = four.w;
+    }
+  }
+  auto for_keys = [&](auto f) {  // f(place among the candidates, key)
+    if constexpr (kKeys > 0) {
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i)
+        if (first + i < candidates) f(first + i, reg[i]);
+    } else {
+      for (int k = first; k < last; ++k) f(k, __ldcg(keys + k));
+    }
+  };
+  for (int k = tid; k < p.sink; k += blockDim.x) out[k] = __ldcg(table + k);
+  for (int k = tid; k < p.local; k += blockDim.x) out[p.budget - p.local + k] = __ldcg(table + v.used - p.local + k);
   if (tid == 0) p.selected_lens[row] = v.len - (v.used - p.budget) * p.page_size;
   if (wanted == 0) return;
-  // the key of the last page that is taken, byte by byte; left: how many of the keys with the bytes so far are still wanted
-  uint32_t prefix = 0, left = wanted;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int k = tid; k < 256; k += kSelThreads) hist_s[k] = 0;
+  uint32_t low = 0xffffffffu, high = 0;
+  for_keys([&](int, uint32_t key) {
+    low = min(low, key);
+    high = max(high, key);
+  });
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) {
+    range_s[0][warp] = low;
+    range_s[1][warp] = high;
+  }
+  __syncthreads();
+  low = __reduce_min_sync(0xffffffffu, range_s[0][lane < warps ? lane : 0]);
+  high = __reduce_max_sync(0xffffffffu, range_s[1][lane < warps ? lane : 0]);
+  // Keys above `high` are fewer than wanted (none, to begin with), keys from `low` on are enough.
+  uint32_t above = 0;  // keys > high
+  for (int turn = 0; low < high; ++turn) {
+    const uint32_t middle = low + (high - low) / 2;
+    uint32_t n = 0;
+    for_keys([&](int, uint32_t key) { n += key > middle; });
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) sum_s[turn & 1][warp] = n;
     __syncthreads();
-    for (int k = tid; k < candidates; k += kSelThreads)
-      if (shift == 24 || (__ldcg(keys + k) >> (shift + 8)) == prefix) atomicAdd(&hist_s[(__ldcg(keys + k) >> shift) & 255], 1);
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t above = 0;
-      int d = 255;
-      while (above + hist_s[d] < left) above += hist_s[d--];
-      digit_s = d;
-      above_s = above;
+    n = __reduce_add_sync(0xffffffffu, lane < warps ? sum_s[turn & 1][lane] : 0u);
+    if (n >= uint32_t(wanted)) {
+      low = middle + 1;
+      if (n == uint32_t(wanted)) {  // these are the ones
+        high = middle;
+        above = n;
+        break;
+      }
+    } else {
+      high = middle;
+      above = n;
     }
-    __syncthreads();
-    prefix = (prefix << 8) | digit_s;
-    left -= above_s;
   }
-  int taken = 0, ties = 0;
-  for (int base = 0; base < candidates; base += kSelThreads) {
-    const int k = base + tid;
-    const uint32_t key = k < candidates ? __ldcg(keys + k) : 0;
-    int n, m;
-    const bool tie = k < candidates && key == prefix;
-    const int before = scan_before(tie, warp_s, &n);
-    const bool take = k < candidates && (key > prefix || (tie && ties + before < int(left)));
-    const int at = scan_before(take, warp_s, &m);
-    if (take) out[p.sink + taken + at] = table[p.sink + k];
-    taken += m;
-    ties += n;
+  // taken: keys > high, and of those equal to it the first wanted - above
+  const uint32_t ties = uint32_t(wanted) - above;
+  uint32_t more = 0, equal = 0;
+  for_keys([&](int, uint32_t key) {
+    more += key > high;
+    equal += key == high;
+  });
+  uint32_t more_before = more, equal_before = equal;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t a = __shfl_up_sync(0xffffffffu, more_before, o), b = __shfl_up_sync(0xffffffffu, equal_before, o);
+    more_before += lane >= o ? a : 0;
+    equal_before += lane >= o ? b : 0;
   }
+  __syncthreads();
+  if (lane == 31) {
+    range_s[0][warp] = more_before;
+    range_s[1][warp] = equal_before;
+  }
+  __syncthreads();
+  more_before += __reduce_add_sync(0xffffffffu, lane < warp ? range_s[0][lane] : 0u) - more;
+  equal_before += __reduce_add_sync(0xffffffffu, lane < warp ? range_s[1][lane] : 0u) - equal;
+  for_keys([&](int k, uint32_t key) {
+    const bool tie = key == high;
+    if (key > high || (tie && equal_before < ties)) out[p.sink + more_before + min(equal_before, ties)] = __ldcg(table + p.sink + k);
+    more_before += key > high;
+    equal_before += tie;
+  });
 }
 
 }  // namespace
@@ -196,7 +239,11 @@ cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream) {
     cudaError_t e = launch_score(p, sms, stream);
     if (e != cudaSuccess) return e;
   }
-  return launch_dependent(select_kernel, dim3(unsigned(p.batch * p.q_len)), kSelThreads, 0, stream, p);
+  // keys of the longest row that the tables can hold: four a thread while there are threads, then sixteen
+  const int rows = p.batch * p.q_len, most = p.width - p.sink - p.local;
+  const int threads = most <= 4 * 256 ? 256 : most <= 4 * 512 ? 512 : kSelMost;
+  const auto kernel = most <= 4 * kSelMost ? select_kernel<4> : most <= 16 * kSelMost ? select_kernel<16> : select_kernel<0>;
+  return launch_dependent(kernel, dim3(unsigned(rows)), threads, 0, stream, p);
 }
 
 }  // namespace mla

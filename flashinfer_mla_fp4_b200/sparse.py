@@ -139,8 +139,8 @@ def select_pages(q: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tenso
 
     ``q`` e4m3 [batch, q_len, H, 576] (strides that are multiples of 16, unit inner stride, H <= 128); ``seq_lens`` int32 [batch].  With ``causal``
     position i of q_len does not see the q_len - 1 - i newest tokens; without it every position sees all of them, as in
-    ``BatchMLADecodeCuteDSLFP4Wrapper.run``.  Entries behind a row's last page are 0.  ``workspace`` (int8, ``4 * batch * q_len * max_pages``
-    bytes, 16-byte aligned; allocated when not given) holds the scores.  Asynchronous on the current stream, capturable."""
+    ``BatchMLADecodeCuteDSLFP4Wrapper.run``.  Entries behind a row's last page are 0.  ``workspace`` (int8, ``4 * batch * q_len`` times
+    max_pages rounded up to a multiple of four; 16-byte aligned; allocated when not given) holds the scores.  Asynchronous on the current stream, capturable."""
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[-1] != HEAD_DIM_QK or q.dtype != torch.float8_e4m3fn:
         raise ValueError(f"q must be an E4M3 tensor [batch, q_len, num_heads, {HEAD_DIM_QK}]")
     if not q.is_cuda:
@@ -291,7 +291,7 @@ def _aligned(n: int) -> int:
 
 
 def _selection_bytes(rows: int, width: int, budget: int) -> int:
-    return _aligned(4 * rows * budget + 4 * rows) + (4 * rows * width if width > budget else 0)
+    return _aligned(4 * rows * budget + 4 * rows) + (_cabi.select_workspace_bytes(rows, 1, width) if width > budget else 0)
 
 
 __all__ = ["BatchMLASparseDecodeFP4Wrapper", "SparsePages", "select_pages", "summarize_new_pages", "summarize_pages"]

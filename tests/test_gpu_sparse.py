@@ -133,6 +133,9 @@ def _selection_case(lens, heads, page, q_len, seed, odd=False):
     ([9000, 100], 64, 64, 1, 1000, 1, 2, False, False),  # a budget beyond the tables
     ([66000, 40000], 17, 8, 1, 600, 3, 5, False, True),
     ([8000, 8001], 33, 8, 1, 990, 3, 5, False, False),  # nearly all
+    ([140000, 131200], 8, 8, 1, 700, 1, 2, False, True),  # more candidates than a CTA's registers hold
+    ([1030] * 1100, 4, 128, 1, 8, 1, 2, False, False),  # more rows than a launch, hardly a tile each
+    ([300, 9000, 17, 1100, 0, 128 * 130], 112, 8, 2, 20, 1, 2, True, True),  # tiles of different rows in turn
 ])
 def test_selection_equals_the_oracle(lens, heads, page, q_len, budget, sink, local, causal, odd):
     dev = _dev()
@@ -146,6 +149,39 @@ def test_selection_equals_the_oracle(lens, heads, page, q_len, budget, sink, loc
     assert torch.equal(got.cpu(), want)
 
 
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right():
+    """A poll budget of one: the first wait for a tile's loads gives up.  What is selected then are pages of the request all the same."""
+    dev = _dev()
+    import ctypes as C
+
+    from flashinfer_mla_fp4_b200 import _cabi
+
+    q, summary, ssf, bt, sl = _selection_case([9000, 700, 12000], 64, 8, 1, seed=3)
+    want, want_lens = S.select(q, summary, ssf, bt, sl, 8, 30, 1, 2, False)
+    qd, summary, ssf, btd, sld = (t.to(dev) for t in (q, summary, ssf, bt, sl))
+    sel, lens = torch.empty(3, 30, dtype=torch.int32, device=dev), torch.empty(3, dtype=torch.int32, device=dev)
+    ws, status = torch.zeros(_cabi.select_workspace_bytes(3, 1, bt.shape[1]), dtype=torch.int8, device=dev), torch.zeros(8, dtype=torch.int32, device=dev)
+    a = _cabi.SelectArgs()
+    a.q, a.q_stride_batch, a.q_stride_qpos, a.q_stride_head = qd.data_ptr(), qd.stride(0), qd.stride(1), qd.stride(2)
+    a.summary, a.summary_sf, a.num_pages = summary.data_ptr(), ssf.data_ptr(), summary.shape[0]
+    a.block_tables, a.block_table_stride, a.seq_lens = btd.data_ptr(), btd.stride(0), sld.data_ptr()
+    a.selected, a.selected_lens, a.workspace, a.workspace_bytes = sel.data_ptr(), lens.data_ptr(), ws.data_ptr(), ws.numel()
+    a.batch, a.q_len, a.num_heads, a.page_size, a.width = 3, 1, 64, 8, bt.shape[1]
+    a.budget, a.sink_pages, a.local_pages, a.status, a.wait_polls = 30, 1, 2, status.data_ptr(), 1
+    a.stream = torch.cuda.current_stream().cuda_stream
+    _cabi.check(_cabi.lib.mla_fp4_select_pages(C.byref(a)))
+    torch.cuda.synchronize()
+    assert int(status[0]) in (0, _cabi.ERR_DEVICE_TIMEOUT)
+    assert torch.equal(lens.cpu(), want_lens)
+    for b in range(3):
+        assert set(sel[b].tolist()) <= set(bt[b].tolist())
+    status.zero_()
+    a.wait_polls = 0
+    _cabi.check(_cabi.lib.mla_fp4_select_pages(C.byref(a)))
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0 and torch.equal(sel.cpu(), want)
+
+
 def test_selection_from_strided_queries_and_tables_into_given_buffers():
     dev = _dev()
     from flashinfer_mla_fp4_b200.sparse import select_pages
@@ -157,7 +193,7 @@ def test_selection_from_strided_queries_and_tables_into_given_buffers():
     wide_bt = torch.full((2, bt.shape[1] + 5), -1, dtype=torch.int32, device=dev)
     wide_bt[:, 2:-3] = bt.to(dev)
     sel, lens = torch.empty(4, 20, dtype=torch.int32, device=dev), torch.empty(4, dtype=torch.int32, device=dev)
-    ws = torch.empty(4 * 4 * bt.shape[1], dtype=torch.int8, device=dev)
+    ws = torch.empty(4 * 4 * ((bt.shape[1] + 3) // 4 * 4), dtype=torch.int8, device=dev)
     got = select_pages(wide_q.view(E4M3)[:, :, 8:32, 32:608], summary.to(dev), ssf.to(dev), wide_bt[:, 2:-3], sl.to(dev), 16, 20,
                        selected=sel, selected_lens=lens, workspace=ws)
     assert got[0] is sel and got[1] is lens

@@ -56,7 +56,7 @@ def test_abi_refuses_before_any_launch():
 
     lib, bad, P = _cabi.lib, _cabi.ERR_BAD_ARG, 4096  # an address that is looked at as a number only
     assert lib.mla_fp4_select_pages(None) == bad
-    assert _cabi.select_workspace_bytes(3, 2, 100) == 3 * 2 * 100 * 4
+    assert _cabi.select_workspace_bytes(3, 2, 98) == 3 * 2 * 100 * 4
     n = C.c_size_t(0)
     assert lib.mla_fp4_select_workspace_bytes(3, 0, 100, C.byref(n)) == bad
 
