@@ -231,7 +231,10 @@ def _load_native():
         raise ImportError(f"the native call path is missing or does not load ({e}): build it with "
                           "`python -m flashinfer_mla_fp4_b200.build`. There is no fallback path.") from e
     names = ("mla_fp4_decode", "mla_fp4_workspace_bytes", "mla_fp4_cache_write", "mla_fp4_step_metadata", "mla_fp4_last_error")
+    sparse = ("mla_fp4_summarize_pages", "mla_fp4_summarize_new_pages", "mla_fp4_select_workspace_bytes", "mla_fp4_select_pages",
+              "mla_fp4_pool_workspace_bytes", "mla_fp4_pool_allocate", "mla_fp4_pool_fork", "mla_fp4_pool_free", "mla_fp4_pool_compact")
     _native.bind(*(C.cast(getattr(lib, n), C.c_void_p).value for n in names))
+    _native.bind_sparse(*(C.cast(getattr(lib, n), C.c_void_p).value for n in sparse))
     return _native
 
 

@@ -15,6 +15,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <string>
 
@@ -36,6 +37,15 @@ struct Abi {
   decltype(&mla_fp4_cache_write) cache_write = nullptr;
   decltype(&mla_fp4_step_metadata) step_metadata = nullptr;
   decltype(&mla_fp4_last_error) last_error = nullptr;
+  decltype(&mla_fp4_summarize_pages) summarize_pages = nullptr;
+  decltype(&mla_fp4_summarize_new_pages) summarize_new_pages = nullptr;
+  decltype(&mla_fp4_select_workspace_bytes) select_workspace_bytes = nullptr;
+  decltype(&mla_fp4_select_pages) select_pages = nullptr;
+  decltype(&mla_fp4_pool_workspace_bytes) pool_workspace_bytes = nullptr;
+  decltype(&mla_fp4_pool_allocate) pool_allocate = nullptr;
+  decltype(&mla_fp4_pool_fork) pool_fork = nullptr;
+  decltype(&mla_fp4_pool_free) pool_free = nullptr;
+  decltype(&mla_fp4_pool_compact) pool_compact = nullptr;
 } abi;
 
 // Without the GIL for as long as it lives.
@@ -59,6 +69,10 @@ PyObject* raise_status(int rc) {
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 bool on(const at::Tensor& t, const at::Device& d) { return t.is_cuda() && t.device() == d; }
+bool validating() {
+  const char* v = std::getenv("MLA_FP4_VALIDATE");
+  return v && *v && !(v[0] == '0' && !v[1]);
+}
 // A number as a double / an integer; anything else (a tensor, say) is left to the Python path.
 bool number(PyObject* o, double* v) {
   if (PyFloat_Check(o)) *v = PyFloat_AS_DOUBLE(o);
@@ -77,19 +91,48 @@ bool integer(PyObject* o, int64_t* v) {
   return overflow == 0;
 }
 
+bool addresses(PyObject* const* a, Py_ssize_t n, Py_ssize_t wanted, void** p) {
+  if (n != wanted) {
+    PyErr_Format(PyExc_TypeError, "bind takes %zd addresses", wanted);
+    return false;
+  }
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    p[i] = PyLong_AsVoidPtr(a[i]);
+    if (!p[i]) {
+      if (!PyErr_Occurred()) PyErr_Format(PyExc_ValueError, "null address");
+      return false;
+    }
+  }
+  return true;
+}
+template <typename F>
+void set(F& f, void* p) { f = reinterpret_cast<F>(p); }
+
 // bind(decode, workspace_bytes, cache_write, step_metadata, last_error): addresses in the loaded library
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 5) return PyErr_Format(PyExc_TypeError, "bind takes 5 addresses");
   void* p[5];
-  for (int i = 0; i < 5; ++i) {
-    p[i] = PyLong_AsVoidPtr(a[i]);
-    if (!p[i]) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "null address");
-  }
-  abi.decode = reinterpret_cast<decltype(abi.decode)>(p[0]);
-  abi.workspace_bytes = reinterpret_cast<decltype(abi.workspace_bytes)>(p[1]);
-  abi.cache_write = reinterpret_cast<decltype(abi.cache_write)>(p[2]);
-  abi.step_metadata = reinterpret_cast<decltype(abi.step_metadata)>(p[3]);
-  abi.last_error = reinterpret_cast<decltype(abi.last_error)>(p[4]);
+  if (!addresses(a, n, 5, p)) return nullptr;
+  set(abi.decode, p[0]);
+  set(abi.workspace_bytes, p[1]);
+  set(abi.cache_write, p[2]);
+  set(abi.step_metadata, p[3]);
+  set(abi.last_error, p[4]);
+  Py_RETURN_NONE;
+}
+// bind_sparse(summarize_pages, summarize_new_pages, select_workspace_bytes, select_pages, pool_workspace_bytes, pool_allocate, pool_fork, pool_free,
+// pool_compact)
+PyObject* bind_sparse(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  void* p[9];
+  if (!addresses(a, n, 9, p)) return nullptr;
+  set(abi.summarize_pages, p[0]);
+  set(abi.summarize_new_pages, p[1]);
+  set(abi.select_workspace_bytes, p[2]);
+  set(abi.select_pages, p[3]);
+  set(abi.pool_workspace_bytes, p[4]);
+  set(abi.pool_allocate, p[5]);
+  set(abi.pool_fork, p[6]);
+  set(abi.pool_free, p[7]);
+  set(abi.pool_compact, p[8]);
   Py_RETURN_NONE;
 }
 
@@ -122,8 +165,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (bt->dim() != 2 || bt->scalar_type() != at::kInt || bt->stride(1) != 1 || bt->size(0) != batch) Py_RETURN_NONE;
   if (sl->dim() != 1 || sl->scalar_type() != at::kInt || sl->size(0) != batch || !sl->is_contiguous()) Py_RETURN_NONE;
   if (max_len <= 0 || max_len > bt->size(1) * page) Py_RETURN_NONE;
-  const char* validate = std::getenv("MLA_FP4_VALIDATE");
-  if (validate && *validate && !(validate[0] == '0' && !validate[1])) Py_RETURN_NONE;  // page ids are checked on the host first
+  if (validating()) Py_RETURN_NONE;  // page ids are checked on the host first
   size_t need = 0;
   if (abi.workspace_bytes(int32_t(batch), int32_t(q_len), int32_t(heads), int32_t(ctas), &need) != MLA_FP4_OK || size_t(ws->numel()) < need)
     Py_RETURN_NONE;
@@ -315,11 +357,327 @@ PyObject* step_metadata(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- sparse decode and the page pool
+// A contiguous tensor of that type, those extents (-1: any) and that device.
+bool plain(const at::Tensor& t, at::ScalarType type, at::IntArrayRef shape, const at::Device& dev) {
+  if (!on(t, dev) || t.scalar_type() != type || size_t(t.dim()) != shape.size() || !t.is_contiguous()) return false;
+  for (size_t i = 0; i < shape.size(); ++i)
+    if (shape[i] >= 0 && t.size(int64_t(i)) != shape[i]) return false;
+  return true;
+}
+bool cache_ok(const at::Tensor& kv, const at::Tensor& sf) {
+  return kv.is_cuda() && kv.dim() == 3 && kv.scalar_type() == at::kByte && kv.size(2) == MLA_FP4_ROW_BYTES && kv.is_contiguous() &&
+         plain(sf, at::kFloat, {kv.size(0), kv.size(1), 1}, kv.device());
+}
+bool summary_ok(const at::Tensor& summary, const at::Tensor& sf, int64_t pages, const at::Device& dev) {
+  return plain(summary, at::kChar, {pages, MLA_FP4_LATENT_DIM + MLA_FP4_ROPE_DIM}, dev) && plain(sf, at::kFloat, {summary.size(0)}, dev);
+}
+bool tables_ok(const at::Tensor& bt, const at::Tensor& sl, const at::Device& dev) {
+  return on(bt, dev) && bt.dim() == 2 && bt.scalar_type() == at::kInt && bt.size(1) > 0 && bt.stride(1) == 1 && bt.stride(0) >= 0 &&
+         bt.size(1) <= INT32_MAX && plain(sl, at::kInt, {bt.size(0)}, dev);
+}
+bool query_ok(const at::Tensor& q) {
+  return q.is_cuda() && q.dim() == 4 && q.scalar_type() == at::kFloat8_e4m3fn && q.size(3) == MLA_FP4_LATENT_DIM + MLA_FP4_ROPE_DIM && q.stride(3) == 1 &&
+         q.size(0) > 0 && q.size(1) > 0 && q.size(2) > 0 && q.size(2) <= 128;
+}
+// summarize(kv_cache, kv_cache_sf, summary, summary_sf, page_ids, block_tables, seq_lens, new_tokens) -> whether it was launched; page_ids, or
+// the other three
+PyObject* summarize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) return PyErr_Format(PyExc_TypeError, "summarize takes 8 arguments");
+  const at::Tensor *kv = tensor(a[0]), *sf = tensor(a[1]), *su = tensor(a[2]), *ssf = tensor(a[3]);
+  if (!kv || !sf || !su || !ssf || !cache_ok(*kv, *sf)) Py_RETURN_FALSE;
+  const at::Device dev = kv->device();
+  const int64_t pages = kv->size(0), page = kv->size(1);
+  if (!summary_ok(*su, *ssf, pages, dev)) Py_RETURN_FALSE;
+  const bool by_id = a[4] != Py_None;
+  const at::Tensor *ids = nullptr, *bt = nullptr, *sl = nullptr;
+  int64_t fresh = 0;
+  if (by_id) {
+    ids = tensor(a[4]);
+    if (!ids || !plain(*ids, at::kInt, {-1}, dev)) Py_RETURN_FALSE;
+  } else {
+    bt = tensor(a[5]);
+    sl = tensor(a[6]);
+    if (!bt || !sl || !integer(a[7], &fresh) || fresh < 0 || fresh > INT32_MAX || !tables_ok(*bt, *sl, dev)) Py_RETURN_FALSE;
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  const void* kv_p = kv->data_ptr();
+  const float* sf_p = static_cast<const float*>(sf->data_ptr());
+  void* su_p = su->data_ptr();
+  float* ssf_p = static_cast<float*>(ssf->data_ptr());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  int rc;
+  {
+    NoGil released;
+    rc = by_id ? abi.summarize_pages(kv_p, sf_p, pages, int32_t(page), static_cast<const int32_t*>(ids->data_ptr()), ids->numel(), su_p, ssf_p, stream)
+               : abi.summarize_new_pages(kv_p, sf_p, pages, int32_t(page), static_cast<const int32_t*>(bt->data_ptr()), bt->stride(0), int32_t(bt->size(1)),
+                                         static_cast<const int32_t*>(sl->data_ptr()), int32_t(bt->size(0)), int32_t(fresh), su_p, ssf_p, stream);
+  }
+  if (rc != MLA_FP4_OK) return raise_status(rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+struct Budget {
+  int64_t budget, sink, local;
+  int causal;
+  // from four Python values; false: not of the common form
+  bool from(PyObject* const* a) {
+    causal = PyObject_IsTrue(a[3]);
+    return integer(a[0], &budget) && integer(a[1], &sink) && integer(a[2], &local) && causal >= 0 && sink >= 0 && local >= 1 && sink <= INT32_MAX &&
+           local <= INT32_MAX && budget <= INT32_MAX && sink + local <= budget;
+  }
+};
+// What both entry points fill in alike.
+MlaFp4SelectArgs select_args(const at::Tensor& q, const at::Tensor& su, const at::Tensor& ssf, const at::Tensor& bt, const at::Tensor& sl, int64_t page,
+                             const Budget& b) {
+  MlaFp4SelectArgs s = {};
+  s.q = q.data_ptr();
+  s.q_stride_batch = q.stride(0); s.q_stride_qpos = q.stride(1); s.q_stride_head = q.stride(2);
+  s.summary = su.data_ptr();
+  s.summary_sf = static_cast<const float*>(ssf.data_ptr());
+  s.num_pages = su.size(0);
+  s.block_tables = static_cast<const int32_t*>(bt.data_ptr());
+  s.block_table_stride = bt.stride(0);
+  s.seq_lens = static_cast<const int32_t*>(sl.data_ptr());
+  s.batch = int32_t(q.size(0)); s.q_len = int32_t(q.size(1)); s.num_heads = int32_t(q.size(2)); s.page_size = int32_t(page);
+  s.width = int32_t(bt.size(1));
+  s.budget = int32_t(b.budget); s.sink_pages = int32_t(b.sink); s.local_pages = int32_t(b.local); s.causal = b.causal;
+  return s;
+}
+
+// select(q, summary, summary_sf, block_tables, seq_lens, page_size, budget, sink_pages, local_pages, causal, selected, selected_lens, workspace)
+// -> (selected, selected_lens), or None when the call is not of the common form
+PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 13) return PyErr_Format(PyExc_TypeError, "select takes 13 arguments");
+  const at::Tensor *q = tensor(a[0]), *su = tensor(a[1]), *ssf = tensor(a[2]), *bt = tensor(a[3]), *sl = tensor(a[4]);
+  int64_t page;
+  Budget b;
+  if (!q || !su || !ssf || !bt || !sl || !integer(a[5], &page) || !b.from(a + 6) || !query_ok(*q)) Py_RETURN_NONE;
+  const at::Device dev = q->device();
+  if (!summary_ok(*su, *ssf, -1, dev) || !tables_ok(*bt, *sl, dev) || bt->size(0) != q->size(0)) Py_RETURN_NONE;
+  const int64_t rows = q->size(0) * q->size(1), width = bt->size(1);
+  at::Tensor out[3];  // the table, the lengths, the workspace
+  for (int i = 0; i < 3; ++i) {
+    if (a[10 + i] == Py_None) continue;
+    const at::Tensor* t = tensor(a[10 + i]);
+    if (!t) Py_RETURN_NONE;
+    out[i] = *t;
+  }
+  size_t need = 0;
+  if (q->size(0) > INT32_MAX || q->size(1) > INT32_MAX || page < 0 || page > 128 ||
+      abi.select_workspace_bytes(int32_t(q->size(0)), int32_t(q->size(1)), int32_t(width), &need) != MLA_FP4_OK)
+    Py_RETURN_NONE;
+  if (width <= b.budget) need = 0;
+  if ((out[0].defined() && !plain(out[0], at::kInt, {rows, b.budget}, dev)) || (out[1].defined() && !plain(out[1], at::kInt, {rows}, dev)) ||
+      (out[2].defined() && (!plain(out[2], at::kChar, {-1}, dev) || size_t(out[2].numel()) < need)))
+    Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(dev);
+  MlaFp4SelectArgs s = select_args(*q, *su, *ssf, *bt, *sl, page, b);
+  s.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  int rc;
+  {
+    NoGil released;
+    const auto ints = at::TensorOptions().dtype(at::kInt).device(dev);
+    if (!out[0].defined()) out[0] = at::empty({rows, b.budget}, ints);
+    if (!out[1].defined()) out[1] = at::empty({rows}, ints);
+    if (!out[2].defined()) out[2] = at::empty({int64_t(need)}, at::TensorOptions().dtype(at::kChar).device(dev));
+    s.selected = static_cast<int32_t*>(out[0].data_ptr());
+    s.selected_lens = static_cast<int32_t*>(out[1].data_ptr());
+    s.workspace = out[2].data_ptr();
+    s.workspace_bytes = size_t(out[2].numel());
+    rc = abi.select_pages(&s);
+  }
+  if (rc != MLA_FP4_OK) return raise_status(rc);
+  PyObject* r[2];
+  for (int i = 0; i < 2; ++i) r[i] = a[10 + i] != Py_None ? Py_NewRef(a[10 + i]) : THPVariable_Wrap(std::move(out[i]));
+  PyObject* both = r[0] && r[1] ? PyTuple_Pack(2, r[0], r[1]) : nullptr;
+  Py_XDECREF(r[0]);
+  Py_XDECREF(r[1]);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// sparse_decode(workspace, status, num_heads, page_size, out_code, num_ctas, pdl, soft_cap, sink, wait_polls, budget, sink_pages, local_pages, causal,
+//               q, kv_cache, block_tables, seq_lens, max_seq_len, softmax_scale, output_scale, out, kv_cache_sf, summary, summary_sf,
+//               return_lse, lse_out)
+// -> out, (out, lse), or None when the call is not of the common form.  The workspace: the decode step's, then from the next multiple of 256 on the
+// selected table and lengths, then from the next one the scores.
+PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 27) return PyErr_Format(PyExc_TypeError, "sparse_decode takes 27 arguments");
+  const at::Tensor *ws = tensor(a[0]), *status = tensor(a[1]), *q = tensor(a[14]), *kv = tensor(a[15]), *bt = tensor(a[16]), *sl = tensor(a[17]),
+                   *sf = tensor(a[22]), *su = tensor(a[23]), *ssf = tensor(a[24]);
+  int64_t heads, page, out_code, ctas, polls, max_len;
+  double cap, scale, out_scale;
+  Budget b;
+  if (!ws || !status || !q || !kv || !bt || !sl || !sf || !su || !ssf || !integer(a[2], &heads) || !integer(a[3], &page) || !integer(a[4], &out_code) ||
+      !integer(a[5], &ctas) || !number(a[7], &cap) || !integer(a[9], &polls) || !b.from(a + 10) || !integer(a[18], &max_len) || !number(a[19], &scale) ||
+      !number(a[20], &out_scale) || !query_ok(*q) || !cache_ok(*kv, *sf) || validating())
+    Py_RETURN_NONE;
+  const at::Device dev = ws->device();
+  if (q->device() != dev || kv->device() != dev || !on(*status, dev) || q->size(2) != heads || kv->size(1) != page || !summary_ok(*su, *ssf, kv->size(0), dev) ||
+      !tables_ok(*bt, *sl, dev) || bt->size(0) != q->size(0))
+    Py_RETURN_NONE;
+  const int64_t batch = q->size(0), q_len = q->size(1), rows = batch * q_len, width = bt->size(1);
+  if (rows > INT32_MAX || (q_len > 1 && batch > 1 && q->stride(0) != q_len * q->stride(1)) || max_len <= 0 || max_len > width * page) Py_RETURN_NONE;
+  const auto aligned = [](size_t v) { return (v + 255) / 256 * 256; };
+  size_t need = 0, scores = 0;
+  if (abi.workspace_bytes(int32_t(rows), 1, int32_t(heads), int32_t(ctas), &need) != MLA_FP4_OK ||
+      abi.select_workspace_bytes(int32_t(rows), 1, int32_t(width), &scores) != MLA_FP4_OK)
+    Py_RETURN_NONE;
+  const size_t table_at = aligned(need), lens_at = table_at + size_t(rows) * size_t(b.budget) * 4, scores_at = table_at + aligned(size_t(rows) * (size_t(b.budget) + 1) * 4);
+  if (size_t(ws->numel()) < scores_at + (width > b.budget ? scores : 0)) Py_RETURN_NONE;
+  const at::ScalarType out_type =
+      out_code == MLA_FP4_OUT_BF16 ? at::kBFloat16 : (out_code == MLA_FP4_OUT_F32 ? at::kFloat : at::kFloat8_e4m3fn);
+  const int64_t shape[4] = {batch, q_len, heads, MLA_FP4_LATENT_DIM};
+  const bool given = a[21] != Py_None;
+  at::Tensor out, lse;
+  if (given) {
+    const at::Tensor* o = tensor(a[21]);
+    if (!o || !plain(*o, out_type, at::IntArrayRef(shape, 4), dev)) Py_RETURN_NONE;
+    out = *o;
+  }
+  const int want_lse = PyObject_IsTrue(a[25]), pdl = PyObject_IsTrue(a[6]);
+  if (want_lse < 0 || pdl < 0) return nullptr;
+  const bool lse_given = want_lse && a[26] != Py_None;
+  if (lse_given) {
+    const at::Tensor* l = tensor(a[26]);
+    if (!l || !plain(*l, at::kFloat, at::IntArrayRef(shape, 3), dev)) Py_RETURN_NONE;
+    lse = *l;
+  }
+  const at::Tensor* sink = a[8] == Py_None ? nullptr : tensor(a[8]);
+  if (a[8] != Py_None && !sink) Py_RETURN_NONE;
+
+  c10::cuda::CUDAGuard guard(dev);
+  char* base = static_cast<char*>(ws->data_ptr());
+  MlaFp4SelectArgs s = select_args(*q, *su, *ssf, *bt, *sl, page, b);
+  s.selected = reinterpret_cast<int32_t*>(base + table_at);
+  s.selected_lens = reinterpret_cast<int32_t*>(base + lens_at);
+  s.workspace = base + scores_at;
+  s.workspace_bytes = size_t(ws->numel()) - scores_at;
+  s.status = static_cast<int32_t*>(status->data_ptr());
+  s.wait_polls = int32_t(polls);
+  s.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  MlaFp4DecodeArgs d = {};
+  d.q = s.q;
+  d.q_stride_batch = q_len == 1 ? s.q_stride_batch : s.q_stride_qpos;
+  d.q_stride_qpos = 16;  // (one position a row: not looked at)
+  d.q_stride_head = s.q_stride_head;
+  d.kv_cache = kv->data_ptr();
+  d.kv_cache_sf = static_cast<const float*>(sf->data_ptr());
+  d.block_tables = s.selected;
+  d.block_table_stride = b.budget;
+  d.seq_lens = s.selected_lens;
+  d.workspace = base;
+  d.workspace_bytes = table_at;
+  d.status = s.status;
+  d.batch = int32_t(rows); d.q_len = 1; d.num_heads = int32_t(heads); d.page_size = int32_t(page);
+  d.num_pages = kv->size(0);
+  d.softmax_scale = float(scale); d.output_scale = float(out_scale);
+  d.out_dtype = int32_t(out_code);
+  d.num_ctas = int32_t(ctas);
+  d.enable_pdl = pdl;
+  d.stream = s.stream;
+  d.max_pages_per_request = s.budget;
+  const int64_t longest = std::min(max_len, b.budget * page);
+  d.max_seq_len = int32_t(std::min<int64_t>(longest, INT32_MAX));
+  d.wait_polls = int32_t(polls);
+  d.logits_soft_cap = float(cap);
+  d.sink = sink ? static_cast<const float*>(sink->data_ptr()) : nullptr;
+  int rc;
+  {
+    NoGil released;
+    if (!given) out = at::empty(at::IntArrayRef(shape, 4), at::TensorOptions().dtype(out_type).device(dev));
+    if (want_lse && !lse_given) lse = at::empty(at::IntArrayRef(shape, 3), at::TensorOptions().dtype(at::kFloat).device(dev));
+    d.out = out.data_ptr();
+    d.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+    rc = abi.select_pages(&s);
+    if (rc == MLA_FP4_OK) rc = abi.decode(&d);
+  }
+  if (rc != MLA_FP4_OK) return raise_status(rc);
+  PyObject* po = given ? Py_NewRef(a[21]) : THPVariable_Wrap(std::move(out));
+  if (!po || !want_lse) return po;
+  PyObject* pl = lse_given ? Py_NewRef(a[26]) : THPVariable_Wrap(std::move(lse));
+  PyObject* both = pl ? PyTuple_Pack(2, po, pl) : nullptr;
+  Py_DECREF(po);
+  Py_XDECREF(pl);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// pool(what, layers, num_layers, page_size, refcounts, status, block_tables, seq_lens, x, y): what is 0 allocate (x: new_lens), 1 fork (parents,
+// children), 2 free (x: rows), 3 compact (x: remap or None); layers is the address of the host array -> remap of a compaction, else True; None
+// when the call is not of the common form
+PyObject* pool(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) return PyErr_Format(PyExc_TypeError, "pool takes 10 arguments");
+  int64_t what, layers, page;
+  const at::Tensor *ref = tensor(a[4]), *status = tensor(a[5]), *bt = tensor(a[6]), *sl = tensor(a[7]), *x = tensor(a[8]), *y = tensor(a[9]);
+  if (!integer(a[0], &what) || !integer(a[2], &layers) || !integer(a[3], &page) || !ref || !status || !bt || !sl) Py_RETURN_NONE;
+  const void* array = PyLong_AsVoidPtr(a[1]);
+  if (!array) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "null address");
+  const at::Device dev = status->device();
+  const int64_t pages = ref->numel(), rows = bt->size(0);
+  if (!plain(*ref, at::kInt, {-1}, dev) || !tables_ok(*bt, *sl, dev) || rows == 0 || rows > INT32_MAX || (rows > 1 && bt->stride(0) < bt->size(1))) Py_RETURN_NONE;
+  int64_t count = 0;
+  if (what == 0) {
+    if (!x || !plain(*x, at::kInt, {rows}, dev)) Py_RETURN_NONE;
+  } else if (what == 1 || what == 2) {
+    if (!x || !plain(*x, at::kInt, {-1}, dev) || x->numel() == 0 || x->numel() > INT32_MAX) Py_RETURN_NONE;
+    count = x->numel();
+    if (what == 1 && (!y || !plain(*y, at::kInt, {count}, dev))) Py_RETURN_NONE;
+  } else if (a[8] != Py_None && (!x || !plain(*x, at::kInt, {pages}, dev))) {
+    Py_RETURN_NONE;
+  }
+  size_t need = 0;
+  if (abi.pool_workspace_bytes(pages, int32_t(rows), int32_t(count), &need) != MLA_FP4_OK) Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(dev);
+  MlaFp4PoolArgs p = {};
+  p.layers = static_cast<const MlaFp4PageLayer*>(array);
+  p.num_layers = int32_t(layers); p.page_size = int32_t(page);
+  p.num_pages = pages;
+  p.refcounts = static_cast<int32_t*>(ref->data_ptr());
+  p.block_tables = static_cast<int32_t*>(bt->data_ptr());
+  p.block_table_stride = bt->stride(0);
+  p.width = int32_t(bt->size(1)); p.rows = int32_t(rows);
+  p.seq_lens = static_cast<int32_t*>(sl->data_ptr());
+  p.workspace_bytes = need;
+  p.status = static_cast<int32_t*>(status->data_ptr());
+  p.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int32_t *xp = x ? static_cast<const int32_t*>(x->data_ptr()) : nullptr, *yp = y ? static_cast<const int32_t*>(y->data_ptr()) : nullptr;
+  at::Tensor remap;
+  int rc;
+  {
+    NoGil released;
+    at::Tensor workspace = at::empty({int64_t(need)}, at::TensorOptions().dtype(at::kChar).device(dev));
+    p.workspace = workspace.data_ptr();
+    if (what == 0) rc = abi.pool_allocate(&p, xp);
+    else if (what == 1) rc = abi.pool_fork(&p, xp, yp, int32_t(count));
+    else if (what == 2) rc = abi.pool_free(&p, xp, int32_t(count));
+    else {
+      remap = x ? *x : at::empty({pages}, at::TensorOptions().dtype(at::kInt).device(dev));
+      rc = abi.pool_compact(&p, static_cast<int32_t*>(remap.data_ptr()));
+    }
+  }
+  if (rc != MLA_FP4_OK) return raise_status(rc);
+  if (what != 3) Py_RETURN_TRUE;
+  return x ? Py_NewRef(a[8]) : THPVariable_Wrap(std::move(remap));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
+    {"bind_sparse", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_sparse)), METH_FASTCALL, nullptr},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, nullptr},
     {"write_tokens", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(write_tokens)), METH_FASTCALL, nullptr},
     {"step_metadata", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(step_metadata)), METH_FASTCALL, nullptr},
+    {"summarize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(summarize)), METH_FASTCALL, nullptr},
+    {"select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(select)), METH_FASTCALL, nullptr},
+    {"sparse_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sparse_decode)), METH_FASTCALL, nullptr},
+    {"pool", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pool)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

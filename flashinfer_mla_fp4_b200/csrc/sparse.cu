@@ -20,115 +20,192 @@ namespace mla {
 namespace {
 
 // ------------------------------------------------------------------------------------------ summaries
-constexpr int kSumThreads = 320;  // 256: latent, four groups of tokens x 64 words of a row; 64: RoPE, four groups x 16 words
+// A CTA per page.  Latent: a thread has eight dims (a 32-bit word of a row) of every fourth pair of tokens; two tokens at a time, their values as
+// signed bytes side by side, go through dp2a with the two 16-bit weights.  RoPE: a thread has four dims of every sixteenth token; sums of eight
+// values of at most 448 in steps of 2^-9 are exact in FP32, and whole numbers of 2^-9 from there on.
+constexpr int kSumThreads = 256, kSumGroups = kSumThreads / 64, kRopeGroups = kSumThreads / 16;
 
-// twice the value of an E2M1 code
-__device__ __forceinline__ int e2m1_twice(uint32_t nibble) {
-  const int m = int((0x0C08060403020100ull >> (8 * (nibble & 7))) & 0xff);
-  return nibble & 8 ? -m : m;
+// bytes of b:a by the selector's nibbles, whose highest bit asks for the byte's sign instead
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t selector) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(selector));
+  return r;
 }
-// 512 times the value of an E4M3 byte (not NaN)
-__device__ __forceinline__ int e4m3_512(uint32_t b) {
-  const int e = (b >> 3) & 15, m = b & 7, v = e ? (8 | m) << (e - 1) : m;
-  return b & 0x80 ? -v : v;
+// 8 codes -> twice their values as signed bytes, codes 0-3 and 4-7
+__device__ __forceinline__ void e2m1x8_twice(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  constexpr uint32_t kP0 = 0x03020100u, kP1 = 0x0C080604u, kN0 = 0xFDFEFF00u, kN1 = 0xF4F8FAFCu;  // 0 1 2 3 4 6 8 12, and negated
+  const uint32_t s0 = w & 0x7777u, s1 = (w >> 16) & 0x7777u, x = w << 4;
+  const uint32_t m0 = prmt(x, w, 0xD9C8u), m1 = prmt(x, w, 0xFBEAu);  // the signs as byte masks
+  lo = (prmt(kP0, kP1, s0) & ~m0) | (prmt(kN0, kN1, s0) & m0);
+  hi = (prmt(kP0, kP1, s1) & ~m1) | (prmt(kN0, kN1, s1) & m1);
 }
+__device__ __forceinline__ int dp2a_lo(int w2, uint32_t b, int c) { return __dp2a_lo(w2, int(b), c); }
+__device__ __forceinline__ int dp2a_hi(int w2, uint32_t b, int c) { return __dp2a_hi(w2, int(b), c); }
 
+template <int kPage>
 __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams p) {
-  __shared__ int w_s[kTile];
-  __shared__ int part_s[4][kQDim];
-  __shared__ float top_s[kSumThreads / 32];
-  __shared__ double amax_s[kSumThreads / 32];
+  constexpr int kWarps = kSumThreads / 32;
+  __shared__ __align__(8) int16_t w_s[kPage];
+  __shared__ int part_s[kSumGroups][kLatent], rope_s[kRopeGroups][kRope];
+  __shared__ float top_s[kWarps];
+  __shared__ int most_s[2][kWarps];
   __shared__ int unsound_s;
   dependent_launch();
-  const int tid = threadIdx.x, n = p.page_size;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int page = -1;
   if (p.page_ids) {
-    page = p.page_ids[blockIdx.x];
+    page = __ldcg(p.page_ids + blockIdx.x);
   } else {  // the pages that the last new_tokens positions of a request have filled, the newest first
     const int b = blockIdx.x / p.per_request, j = blockIdx.x - b * p.per_request;
-    const int len = min(p.seq_lens[b], p.seq_cap), at = len / n - 1 - j;
-    if (at >= 0 && (at + 1) * int64_t(n) > int64_t(len) - p.new_tokens) page = p.block_tables[int64_t(b) * p.block_table_stride + at];
+    const int len = min(__ldcg(p.seq_lens + b), p.seq_cap), at = len / kPage - 1 - j;
+    if (at >= 0 && (at + 1) * int64_t(kPage) > int64_t(len) - p.new_tokens) page = __ldcg(p.block_tables + int64_t(b) * p.block_table_stride + at);
   }
   if (page < 0 || page >= p.num_pages) return;
-  const uint8_t* rows = p.kv_cache + int64_t(page) * n * kRowBytes;
-  const float* sf = p.kv_cache_sf + int64_t(page) * n;
-  const float s = tid < n ? sf[tid] : 0.f;
+  const uint8_t* rows = p.kv_cache + int64_t(page) * kPage * kRowBytes;
+  const float s = tid < kPage ? __ldcg(p.kv_cache_sf + int64_t(page) * kPage + tid) : 0.f;
+  // all of the page is asked for before anything is done with it
+  constexpr int kPairs = kPage / 2, kMine = (kPairs + kSumGroups - 1) / kSumGroups, kRopeMine = (kPage + kRopeGroups - 1) / kRopeGroups;
+  const int word = tid & 63, group = tid >> 6;
+  uint32_t v[kMine][2], r[kRopeMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int pair = group + i * kSumGroups;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) v[i][k] = pair < kPairs ? __ldcg(reinterpret_cast<const uint32_t*>(rows + (2 * pair + k) * kRowBytes) + word) : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < kRopeMine; ++i) {
+    const int t = (tid >> 4) + i * kRopeGroups;
+    r[i] = t < kPage ? __ldcg(reinterpret_cast<const uint32_t*>(rows + t * kRowBytes + kLatent / 2) + (tid & 15)) : 0u;
+  }
   float top = fabsf(s);
-  int unsound = !(top <= CUDART_MAX_NORMAL_F);
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  bool unsound = !(top <= CUDART_MAX_NORMAL_F);
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(unsound ? 0.f : top)));  // (non-negative floats order as integers)
   if (tid == 0) unsound_s = 0;
-  if ((tid & 31) == 0) top_s[tid >> 5] = top;
+  if (lane == 0) top_s[warp] = top;
   __syncthreads();
-  top = 0.f;
-  for (int i = 0; i < kSumThreads / 32; ++i) top = fmaxf(top, top_s[i]);
-  if (tid < n) w_s[tid] = top > 0.f && !unsound ? int(rint(32767.0 * double(s) / double(top))) : 0;
+#pragma unroll
+  for (int i = 0; i < (kPage + 31) / 32; ++i) top = fmaxf(top, top_s[i]);
   if (unsound) unsound_s = 1;
+  if (tid < kPage) w_s[tid] = top > 0.f && !unsound ? int16_t(rint(32767.0 * double(s) / double(top))) : int16_t(0);
+  // RoPE meanwhile: nobody waits for the weights
+  float sum[4] = {};
+#pragma unroll
+  for (int i = 0; i < kRopeMine; ++i) {
+    const float2 a = e4m3x2_to_float2(r[i] & 0xffff), b = e4m3x2_to_float2(r[i] >> 16);
+    sum[0] += a.x;
+    sum[1] += a.y;
+    sum[2] += b.x;
+    sum[3] += b.y;
+  }
+  const bool nan = !(sum[0] == sum[0] && sum[1] == sum[1] && sum[2] == sum[2] && sum[3] == sum[3]);
+  if (nan) unsound_s = 1;
+  *reinterpret_cast<int4*>(&rope_s[tid >> 4][4 * (tid & 15)]) =
+      make_int4(int(512.f * sum[0]), int(512.f * sum[1]), int(512.f * sum[2]), int(512.f * sum[3]));
   __syncthreads();
-  if (tid < 256) {
-    const int c = tid & 63;
-    int acc[8] = {};
-    for (int t = tid >> 6; t < n; t += 4) {
-      const uint32_t v = *reinterpret_cast<const uint32_t*>(rows + t * kRowBytes + 4 * c);
-      const int w = w_s[t];
+  int acc[8] = {};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += w * e2m1_twice(v >> (4 * i));
-    }
-    for (int i = 0; i < 8; ++i) part_s[tid >> 6][8 * c + i] = acc[i];
-  } else {
-    const int c = tid & 15, g = (tid - 256) >> 4;
-    int acc[4] = {};
-    for (int t = g; t < n; t += 4) {
-      const uint32_t v = *reinterpret_cast<const uint32_t*>(rows + t * kRowBytes + kLatent / 2 + 4 * c);
+  for (int i = 0; i < kMine; ++i) {
+    const int pair = group + i * kSumGroups;
+    const int w2 = pair < kPairs ? *reinterpret_cast<const int*>(w_s + 2 * pair) : 0;
+    uint32_t a0, a1, b0, b1;
+    e2m1x8_twice(v[i][0], a0, a1);
+    e2m1x8_twice(v[i][1], b0, b1);
+    const uint32_t p01 = __byte_perm(a0, b0, 0x5140), p23 = __byte_perm(a0, b0, 0x7362), p45 = __byte_perm(a1, b1, 0x5140), p67 = __byte_perm(a1, b1, 0x7362);
+    acc[0] = dp2a_lo(w2, p01, acc[0]);
+    acc[1] = dp2a_hi(w2, p01, acc[1]);
+    acc[2] = dp2a_lo(w2, p23, acc[2]);
+    acc[3] = dp2a_hi(w2, p23, acc[3]);
+    acc[4] = dp2a_lo(w2, p45, acc[4]);
+    acc[5] = dp2a_hi(w2, p45, acc[5]);
+    acc[6] = dp2a_lo(w2, p67, acc[6]);
+    acc[7] = dp2a_hi(w2, p67, acc[7]);
+  }
+  // (eight words each: the two halves of a row's words go to the banks side by side)
+  *reinterpret_cast<int4*>(&part_s[group][4 * word]) = make_int4(acc[0], acc[1], acc[2], acc[3]);
+  *reinterpret_cast<int4*>(&part_s[group][kLatent / 2 + 4 * word]) = make_int4(acc[4], acc[5], acc[6], acc[7]);
+  __syncthreads();
+  // a thread has dims 8 w + 2 k, + 1 (w, k: its pair's place above), the first 32 threads two of RoPE too
+  const int place = 2 * tid;  // in part_s: half h of word w at h * 256 + 4 w + j
+  const int dim = place < kLatent / 2 ? (place >> 2) * 8 + (place & 3) : ((place - kLatent / 2) >> 2) * 8 + 4 + (place & 3);
+  int2 lat = *reinterpret_cast<const int2*>(&part_s[0][place]), rope = make_int2(0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t b = (v >> (8 * i)) & 0xff;
-        if ((b & 0x7f) == 0x7f) unsound = 1;
-        else acc[i] += e4m3_512(b);
-      }
+  for (int g = 1; g < kSumGroups; ++g) {
+    const int2 more = *reinterpret_cast<const int2*>(&part_s[g][place]);
+    lat.x += more.x;
+    lat.y += more.y;
+  }
+  if (tid < kRope / 2)
+#pragma unroll
+    for (int g = 0; g < kRopeGroups; ++g) {
+      const int2 more = *reinterpret_cast<const int2*>(&rope_s[g][2 * tid]);
+      rope.x += more.x;
+      rope.y += more.y;
     }
-    for (int i = 0; i < 4; ++i) part_s[g][kLatent + 4 * c + i] = acc[i];
-    if (unsound) unsound_s = 1;
+  const int most_lat = __reduce_max_sync(0xffffffffu, max(abs(lat.x), abs(lat.y))), most_rope = __reduce_max_sync(0xffffffffu, max(abs(rope.x), abs(rope.y)));
+  if (lane == 0) {
+    most_s[0][warp] = most_lat;
+    most_s[1][warp] = most_rope;
   }
   __syncthreads();
-  const double lat = double(top) / (65534.0 * n), rope = 1.0 / (512.0 * n);
-  double mean[2], amax = 0;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int d = tid + k * kSumThreads;
-    mean[k] = d < kQDim ? double(part_s[0][d] + part_s[1][d] + part_s[2][d] + part_s[3][d]) * (d < kLatent ? lat : rope) : 0.0;
-    amax = fmax(amax, fabs(mean[k]));
-  }
-  for (int o = 16; o > 0; o >>= 1) amax = fmax(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((tid & 31) == 0) amax_s[tid >> 5] = amax;
-  __syncthreads();
-  for (int i = 0; i < kSumThreads / 32; ++i) amax = fmax(amax, amax_s[i]);
-  const float scale = float(amax / 127.0);
-  const bool sound = !unsound_s && scale <= CUDART_MAX_NORMAL_F;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int d = tid + k * kSumThreads;
-    if (d < kQDim) p.summary[int64_t(page) * kQDim + d] = sound && scale > 0.f ? int8_t(fmin(fmax(rint(mean[k] / double(scale)), -127.0), 127.0)) : int8_t(0);
+  const int ml = __reduce_max_sync(0xffffffffu, most_s[0][lane & (kWarps - 1)]), mr = most_s[1][0];
+  const double of_lat = double(top) / (65534.0 * kPage), of_rope = 1.0 / (512.0 * kPage);
+  const float scale = float(fmax(double(ml) * of_lat, double(mr) * of_rope) / 127.0);
+  const bool sound = !unsound_s && scale <= CUDART_MAX_NORMAL_F, some = sound && scale > 0.f;
+  // Codes in FP32 unless that is too near the middle of two: the product is off by less than 2^-16 (three roundings of at most 127 ulp-halves).
+  const float lat32 = float(of_lat / double(scale)), rope32 = float(of_rope / double(scale));
+  auto code = [&](int sum_of, float by32, double by) -> int {
+    if (!some) return 0;
+    const float x = float(sum_of) * by32, whole = rintf(x);
+    if (fabsf(fabsf(x - whole) - 0.5f) > 0x1p-12f && fabsf(x) < 130.f) return min(max(int(whole), -127), 127);
+    return int(fmin(fmax(rint(double(sum_of) * by / double(scale)), -127.0), 127.0));
+  };
+  char* out = reinterpret_cast<char*>(p.summary) + int64_t(page) * kQDim;
+  const int c0 = code(lat.x, lat32, of_lat), c1 = code(lat.y, lat32, of_lat);
+  *reinterpret_cast<uint16_t*>(out + dim) = uint16_t((c0 & 0xff) | (c1 & 0xff) << 8);
+  if (tid < kRope / 2) {
+    const int r0 = code(rope.x, rope32, of_rope), r1 = code(rope.y, rope32, of_rope);
+    *reinterpret_cast<uint16_t*>(out + kLatent + 2 * tid) = uint16_t((r0 & 0xff) | (r1 & 0xff) << 8);
   }
   if (tid == 0) p.summary_sf[page] = sound ? scale : CUDART_NAN_F;
 }
 
 // ------------------------------------------------------------------------------------------ selection
-// A CTA per row.  A thread has kKeys consecutive keys in registers; the key of the last page that is taken is found by halving the range of the
-// keys until as many lie above the middle as are wanted, which takes about log2(candidates) + 2 counts, 32 where pages tie: a count is a
-// compare per key, a reduction in the warp and one across warps behind one barrier.  (By bytes through a histogram in shared memory, whose
-// counters of the leading byte everybody wants, 2045 of 64 rows took 39 us.)  Then one scan gives each page that is taken its place.
-// kKeys = 0: more candidates than registers hold; the keys stay in global memory, read through L2 at each count.
-constexpr int kSelMost = 1024;
+// A CTA per row.  A thread has kKeys consecutive keys in registers (and their block-table entries: all loads of a row are on their way at once,
+// before its length is known).  The key of the last page that is taken is found by counting the keys' range in 256 buckets, going on with the
+// bucket in which the count reaches what is wanted: two rounds where keys are spread, four where they are not or pages tie.
+// Then one scan gives each page that is taken its place.  64 rows of 2048 pages, nothing in L2: 39.8 us by bytes of the keys, whose leading
+// byte is nearly everybody's, so that all threads wanted the same counter; 9.8 by halving the range with a barrier each time; 6.7 so.
+// kKeys = 0: more candidates than registers hold; the keys stay in global memory and are read through L2 in each round.
+constexpr int kSelMost = 1024, kBuckets = 256;
 
 template <int kKeys>
 __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
-  __shared__ uint32_t sum_s[2][32], range_s[2][32];
+  __shared__ uint32_t range_s[2][32], bucket_s[kBuckets], found_s[3];
   dependent_launch();
   const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
   const uint32_t* keys = p.keys + int64_t(row) * p.key_stride;
-  const Seen v = seen(p, row);
   const int32_t* table = p.block_tables + int64_t(row / p.q_len) * p.block_table_stride;
   int32_t* out = p.selected + int64_t(row) * p.budget;
+  uint32_t reg[kKeys ? kKeys : 1];
+  constexpr bool kPagesToo = kKeys == 4;  // (with sixteen there are no registers for them)
+  int32_t page[kPagesToo ? kKeys : 1];
+  if constexpr (kKeys > 0) {
+#pragma unroll
+    for (int i = 0; i < kKeys; i += 4) {  // (a row has room for whole groups of four; what lies behind the candidates is not looked at)
+      const int k = tid * kKeys + i;
+      if (k >= p.width) break;
+      const uint4 four = __ldcg(reinterpret_cast<const uint4*>(keys + k));
+      reg[i] = four.x;
+      reg[i + 1] = four.y;
+      reg[i + 2] = four.z;
+      reg[i + 3] = four.w;
+      if constexpr (kPagesToo)
+#pragma unroll
+        for (int j = i; j < i + 4; ++j) page[j] = p.sink + tid * kKeys + j < p.width ? __ldcg(table + p.sink + tid * kKeys + j) : 0;
+    }
+  }
+  const Seen v = seen(p, row);
   if (v.used <= p.budget) {  // the budget holds them all
     for (int k = tid; k < p.budget; k += blockDim.x) out[k] = k < v.used ? __ldcg(table + k) : 0;
     if (tid == 0) p.selected_lens[row] = v.len;
@@ -137,25 +214,13 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
   const int candidates = v.used - p.sink - p.local, wanted = p.budget - p.sink - p.local;
   const int mine = kKeys ? kKeys : (candidates + int(blockDim.x) - 1) / int(blockDim.x);
   const int first = tid * mine, last = min(first + mine, candidates);
-  uint32_t reg[kKeys ? kKeys : 1];
-  if constexpr (kKeys > 0) {
-#pragma unroll
-    for (int i = 0; i < kKeys; i += 4) {  // (a row has room for whole groups of four; what lies behind the candidates is not looked at)
-      if (first + i >= candidates) break;
-      const uint4 four = __ldcg(reinterpret_cast<const uint4*>(keys + first + i));
-      reg[i] = four.x;
-      reg[i + 1] = four.y;
-      reg[i + 2] = four.z;
-      reg[i + 3] = four.w;
-    }
-  }
-  auto for_keys = [&](auto f) {  // f(place among the candidates, key)
+  auto for_keys = [&](auto f) {  // f(key, its page when called)
     if constexpr (kKeys > 0) {
 #pragma unroll
       for (int i = 0; i < kKeys; ++i)
-        if (first + i < candidates) f(first + i, reg[i]);
+        if (first + i < candidates) f(reg[i], [&] { return kPagesToo ? page[kPagesToo ? i : 0] : __ldcg(table + p.sink + first + i); });
     } else {
-      for (int k = first; k < last; ++k) f(k, __ldcg(keys + k));
+      for (int k = first; k < last; ++k) f(__ldcg(keys + k), [&] { return __ldcg(table + p.sink + k); });
     }
   };
   for (int k = tid; k < p.sink; k += blockDim.x) out[k] = __ldcg(table + k);
@@ -163,7 +228,7 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
   if (tid == 0) p.selected_lens[row] = v.len - (v.used - p.budget) * p.page_size;
   if (wanted == 0) return;
   uint32_t low = 0xffffffffu, high = 0;
-  for_keys([&](int, uint32_t key) {
+  for_keys([&](uint32_t key, auto) {
     low = min(low, key);
     high = max(high, key);
   });
@@ -173,35 +238,62 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
     range_s[0][warp] = low;
     range_s[1][warp] = high;
   }
+  for (int k = tid; k < kBuckets; k += blockDim.x) bucket_s[k] = 0;
   __syncthreads();
   low = __reduce_min_sync(0xffffffffu, range_s[0][lane < warps ? lane : 0]);
   high = __reduce_max_sync(0xffffffffu, range_s[1][lane < warps ? lane : 0]);
   // Keys above `high` are fewer than wanted (none, to begin with), keys from `low` on are enough.
   uint32_t above = 0;  // keys > high
-  for (int turn = 0; low < high; ++turn) {
-    const uint32_t middle = low + (high - low) / 2;
-    uint32_t n = 0;
-    for_keys([&](int, uint32_t key) { n += key > middle; });
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) sum_s[turn & 1][warp] = n;
+  while (low < high) {
+    const int shift = max(0, 24 - __clz(high - low));  // 256 buckets hold the range
+    for_keys([&](uint32_t key, auto) {
+      if (key >= low && key <= high) atomicAdd(&bucket_s[(key - low) >> shift], 1u);
+    });
     __syncthreads();
-    n = __reduce_add_sync(0xffffffffu, lane < warps ? sum_s[turn & 1][lane] : 0u);
-    if (n >= uint32_t(wanted)) {
-      low = middle + 1;
-      if (n == uint32_t(wanted)) {  // these are the ones
-        high = middle;
-        above = n;
-        break;
+    if (warp == 0) {  // lane i has the buckets 8 i to 8 i + 7: the one, from above, in which the count reaches what is wanted
+      uint32_t n[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        n[i] = bucket_s[8 * lane + i];
+        sum += n[i];
+        bucket_s[8 * lane + i] = 0;
       }
-    } else {
-      high = middle;
-      above = n;
+      uint32_t from = sum;  // of this lane and those above it
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t a = __shfl_down_sync(0xffffffffu, from, o);
+        from += lane + o < 32 ? a : 0;
+      }
+      uint32_t over = above + from - sum;
+      if (over < uint32_t(wanted) && over + sum >= uint32_t(wanted)) {
+        bool found = false;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+          if (!found && over + n[i] >= uint32_t(wanted)) {
+            found = true;
+            found_s[0] = 8 * lane + i;
+            found_s[1] = over;
+            found_s[2] = n[i];
+          }
+          over += n[i];
+        }
+      }
     }
+    __syncthreads();
+    const uint32_t bucket = found_s[0], start = low + (bucket << shift);
+    above = found_s[1];
+    if (above + found_s[2] == uint32_t(wanted)) {  // the whole bucket is taken: these are the ones
+      high = start - 1;
+      above = wanted;
+      break;
+    }
+    high = start + min(high - start, (1u << shift) - 1);  // (the bucket's end may lie beyond 32 bits)
+    low = start;
   }
   // taken: keys > high, and of those equal to it the first wanted - above
   const uint32_t ties = uint32_t(wanted) - above;
   uint32_t more = 0, equal = 0;
-  for_keys([&](int, uint32_t key) {
+  for_keys([&](uint32_t key, auto) {
     more += key > high;
     equal += key == high;
   });
@@ -220,9 +312,9 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
   __syncthreads();
   more_before += __reduce_add_sync(0xffffffffu, lane < warp ? range_s[0][lane] : 0u) - more;
   equal_before += __reduce_add_sync(0xffffffffu, lane < warp ? range_s[1][lane] : 0u) - equal;
-  for_keys([&](int k, uint32_t key) {
+  for_keys([&](uint32_t key, auto page_of) {
     const bool tie = key == high;
-    if (key > high || (tie && equal_before < ties)) out[p.sink + more_before + min(equal_before, ties)] = __ldcg(table + p.sink + k);
+    if (key > high || (tie && equal_before < ties)) out[p.sink + more_before + min(equal_before, ties)] = page_of();
     more_before += key > high;
     equal_before += tie;
   });
@@ -231,7 +323,9 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
 }  // namespace
 
 cudaError_t launch_summarize(const SummarizeParams& p, int64_t ctas, cudaStream_t stream) {
-  return launch_dependent(summarize_kernel, dim3(unsigned(ctas)), kSumThreads, 0, stream, p);
+  const auto kernel = p.page_size == 8 ? summarize_kernel<8> : p.page_size == 16 ? summarize_kernel<16> : p.page_size == 32 ? summarize_kernel<32>
+                      : p.page_size == 64 ? summarize_kernel<64> : summarize_kernel<128>;
+  return launch_dependent(kernel, dim3(unsigned(ctas)), kSumThreads, 0, stream, p);
 }
 
 cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream) {
@@ -239,10 +333,10 @@ cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream) {
     cudaError_t e = launch_score(p, sms, stream);
     if (e != cudaSuccess) return e;
   }
-  // keys of the longest row that the tables can hold: four a thread while there are threads, then sixteen
+  // keys of the longest row that the tables can hold: four a thread while there are threads, then sixteen (none where the budget holds every row)
   const int rows = p.batch * p.q_len, most = p.width - p.sink - p.local;
   const int threads = most <= 4 * 256 ? 256 : most <= 4 * 512 ? 512 : kSelMost;
-  const auto kernel = most <= 4 * kSelMost ? select_kernel<4> : most <= 16 * kSelMost ? select_kernel<16> : select_kernel<0>;
+  const auto kernel = p.width <= p.budget ? select_kernel<0> : most <= 4 * kSelMost ? select_kernel<4> : most <= 16 * kSelMost ? select_kernel<16> : select_kernel<0>;
   return launch_dependent(kernel, dim3(unsigned(rows)), threads, 0, stream, p);
 }
 

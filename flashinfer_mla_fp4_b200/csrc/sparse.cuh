@@ -1,6 +1,8 @@
 // What the kernels of sparse decode and of the page pool share.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "launch.h"
 
@@ -25,6 +27,16 @@ cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 b;\n\tcvt.u16.u32 b, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(two_bytes));
+  return r;
+}
+__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two_bytes) {
+  const uint32_t h = e4m3x2_to_f16x2(two_bytes);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
 // What a query position sees of its request.

@@ -84,6 +84,10 @@ class FP4MLAPagePool:
         self.refcounts = torch.zeros(self.num_pages, dtype=torch.int32, device=self.device)
         self._status = torch.zeros(8, dtype=torch.int32, device=self.device)
 
+    def _native(self, what: int, block_tables, seq_lens, x, y=None):
+        """The common form of a call, checked and launched natively; None: nothing was done."""
+        return _cabi.native.pool(what, C.addressof(self._array), len(self._array), self.page_size, self.refcounts, self._status, block_tables, seq_lens, x, y)
+
     def num_free(self) -> int:
         """Free pages (synchronises)."""
         return int((self.refcounts <= 0).sum())
@@ -109,6 +113,8 @@ class FP4MLAPagePool:
         """Give each row the pages that ``new_lens`` (int32 [rows]) tokens take beyond those for ``seq_lens``; the lengths stay as they are.
 
         Rows are served in order.  One that no longer fits into the pool, or into its block-table row, gets nothing."""
+        if self._native(0, block_tables, seq_lens, new_lens) is not None:
+            return
         check_tables(block_tables, seq_lens, self.device)
         check_tensor("new_lens", new_lens, torch.int32, (block_tables.shape[0],), self.device)
         if block_tables.shape[0] == 0:
@@ -123,6 +129,8 @@ class FP4MLAPagePool:
 
         A child's row must be empty (length 0); a parent may have many children.  A fork for which the pool has no page, into a row that is not
         empty, or of a child that the list has named before, is not made."""
+        if self._native(1, block_tables, seq_lens, parents, children) is not None:
+            return
         check_tensor("parents", parents, torch.int32, (None,), self.device)
         check_tensor("children", children, torch.int32, (parents.shape[0],), self.device)
         if parents.numel() == 0:
@@ -134,6 +142,8 @@ class FP4MLAPagePool:
     @api_logged
     def free(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, rows: torch.Tensor) -> None:
         """Take a reference from every page of the rows and set their lengths to 0 (a row that is named twice is freed once)."""
+        if self._native(2, block_tables, seq_lens, rows) is not None:
+            return
         check_tensor("rows", rows, torch.int32, (None,), self.device)
         if rows.numel() == 0:
             return
@@ -147,6 +157,9 @@ class FP4MLAPagePool:
 
         Reference counts and the block tables' entries (as far as ``seq_lens`` says) follow.  Returns ``remap`` int32 [pages]: the new number of
         each page, -1 for one that was free, for whatever else names pages."""
+        done = self._native(3, block_tables, seq_lens, remap)
+        if done is not None:
+            return done
         if remap is None:
             remap = torch.empty(self.num_pages, dtype=torch.int32, device=self.device)
         else:

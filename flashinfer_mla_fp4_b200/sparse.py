@@ -20,6 +20,7 @@ binade's 1/64: NaN first, ties to the page nearer the start.  Dots are of intege
 from __future__ import annotations
 
 import ctypes as C
+import os
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
@@ -28,9 +29,10 @@ import torch
 from . import _cabi
 from .api_log import api_logged
 from .kvcache import HEAD_DIM_QK, ROW_BYTES
-from .wrapper import BatchMLADecodeCuteDSLFP4Wrapper
+from .wrapper import BatchMLADecodeCuteDSLFP4Wrapper, validate_page_ids
 
 PAGE_SIZES = (8, 16, 32, 64, 128)
+_native = _cabi.native
 
 
 @dataclass(frozen=True)
@@ -94,6 +96,8 @@ def summarize_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summary: 
     (int32, contiguous, on the device; those outside the pool are skipped, one that is named twice is written twice alike).
 
     All ``page_size`` rows of a page enter its summary, so call it for pages that are full.  Asynchronous on the current stream."""
+    if _native.summarize(kv_cache, kv_cache_sf, summary, summary_sf, page_ids, None, None, 0):
+        return  # the common form, checked and launched natively; otherwise nothing was done
     pages, page_size = check_cache(kv_cache, kv_cache_sf)
     dev = kv_cache.device
     check_summary(summary, summary_sf, pages, dev)
@@ -113,6 +117,8 @@ def summarize_new_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summa
 
     ``seq_lens`` (int32 [batch]) counts the new tokens, ``block_tables`` int32 [batch, max_pages].  What a step calls behind
     ``write_tokens``; a page that the step has not filled is left alone.  Asynchronous on the current stream."""
+    if _native.summarize(kv_cache, kv_cache_sf, summary, summary_sf, None, block_tables, seq_lens, new_tokens):
+        return
     pages, page_size = check_cache(kv_cache, kv_cache_sf)
     dev = kv_cache.device
     check_summary(summary, summary_sf, pages, dev)
@@ -141,6 +147,10 @@ def select_pages(q: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tenso
     position i of q_len does not see the q_len - 1 - i newest tokens; without it every position sees all of them, as in
     ``BatchMLADecodeCuteDSLFP4Wrapper.run``.  Entries behind a row's last page are 0.  ``workspace`` (int8, ``4 * batch * q_len`` times
     max_pages rounded up to a multiple of four; 16-byte aligned; allocated when not given) holds the scores.  Asynchronous on the current stream, capturable."""
+    done = _native.select(q, summary, summary_sf, block_tables, seq_lens, page_size, budget_pages, sink_pages, local_pages, causal,
+                          selected, selected_lens, workspace)
+    if done is not None:
+        return done
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[-1] != HEAD_DIM_QK or q.dtype != torch.float8_e4m3fn:
         raise ValueError(f"q must be an E4M3 tensor [batch, q_len, num_heads, {HEAD_DIM_QK}]")
     if not q.is_cuda:
@@ -229,7 +239,13 @@ class BatchMLASparseDecodeFP4Wrapper:
         were attended to) are as there."""
         if self._pages is None:
             raise RuntimeError("Call plan() before run().")
-        sp = self._pages
+        sp, dense = self._pages, self._dense
+        done = _native.sparse_decode(self._workspace_buffer, dense._status, self._num_heads, self._page_size, dense._out_code, dense._num_ctas,
+                                     dense._enable_pdl, dense._soft_cap, dense._sink, dense._wait_polls, sp.budget_pages, sp.sink_pages, sp.local_pages,
+                                     sp.causal, q, kv_cache, block_tables, seq_lens, max_seq_len, softmax_scale, output_scale, out, kv_cache_sf,
+                                     summary, summary_sf, return_lse, lse_out)
+        if done is not None:
+            return done
         if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[2] != self._num_heads or q.shape[3] != HEAD_DIM_QK:
             raise ValueError(f"q must have shape [batch, q_len, {self._num_heads}, {HEAD_DIM_QK}]")
         if q.device != self._device:
@@ -254,6 +270,8 @@ class BatchMLASparseDecodeFP4Wrapper:
             raise ValueError("out must be a contiguous [batch, q_len, num_heads, 512] tensor")
         if lse_out is not None and (tuple(lse_out.shape) != shape[:3] or not lse_out.is_contiguous()):
             raise ValueError("lse_out must be a contiguous float32 [batch, q_len, num_heads] tensor on the device of q")
+        if os.environ.get("MLA_FP4_VALIDATE", "0") not in ("", "0"):
+            validate_page_ids(block_tables, seq_lens, page_size, pages)
         rows = batch * q_len
         selected, selected_lens, scores = self._scratch(rows, width)
         select_pages(q, summary, summary_sf, block_tables, seq_lens, page_size, sp.budget_pages, sink_pages=sp.sink_pages,

@@ -149,6 +149,38 @@ def test_selection_equals_the_oracle(lens, heads, page, q_len, budget, sink, loc
     assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("pages", [40, 3000, 17000])
+@pytest.mark.parametrize("shape", ["negative", "negative and NaN", "two values", "one value", "one page stands out", "infinite"])
+def test_selection_over_scores_of_any_spread(pages, shape):
+    """Scores made to order: a summary with one code, a query with one value."""
+    dev = _dev()
+    from flashinfer_mla_fp4_b200.sparse import select_pages
+
+    g = torch.Generator().manual_seed(pages)
+    summary, ssf = torch.zeros(pages, 576, dtype=torch.int8), torch.ones(pages)
+    summary[:, 7] = 1
+    q = torch.zeros(1, 1, 1, 576)
+    q[..., 7] = 2.0
+    if shape.startswith("negative"):
+        ssf = -torch.rand(pages, generator=g) * 10.0 ** torch.randint(-30, 30, (pages,), generator=g)
+        if shape != "negative":
+            ssf[torch.randperm(pages, generator=g)[: pages // 9]] = math.nan
+    elif shape == "two values":
+        ssf[torch.randperm(pages, generator=g)[: pages // 2]] = 1.0 + 2.0 ** -23
+    elif shape == "one page stands out":
+        ssf[pages // 2] = 2.0
+    elif shape == "infinite":
+        ssf[3], ssf[5], summary[9, 7] = math.inf, -math.inf, 0
+        ssf[9] = math.inf  # times zero: NaN
+    bt = torch.randperm(pages, generator=g).int().view(1, -1)
+    sl = torch.tensor([pages * 8 - 3], dtype=torch.int32)
+    want, want_lens = S.select(q.to(E4M3), summary, ssf, bt, sl, 8, 20, 1, 2, False)
+    room = torch.full((1 + pages // 20 + 1, 20), -9, dtype=torch.int32, device=dev)
+    got, lens = select_pages(q.to(E4M3).to(dev), summary.to(dev), ssf.to(dev), bt.to(dev), sl.to(dev), 8, 20, selected=room[:1])
+    assert torch.equal(got.cpu(), want) and torch.equal(lens.cpu(), want_lens)
+    assert bool((room[1:] == -9).all())
+
+
 def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right():
     """A poll budget of one: the first wait for a tile's loads gives up.  What is selected then are pages of the request all the same."""
     dev = _dev()
