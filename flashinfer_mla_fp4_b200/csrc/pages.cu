@@ -77,8 +77,20 @@ __device__ __forceinline__ int for_free_pages(const int32_t* refcounts, int64_t 
 }
 
 // ------------------------------------------------------------------------------------------ copying
+// Five loads of a thread are on their way before the first store (a page of 64 tokens is five rounds of the CTA).
 __device__ __forceinline__ void copy16(void* dst, const void* src, int n16) {
-  for (int i = threadIdx.x; i < n16; i += kMoveThreads) static_cast<uint4*>(dst)[i] = static_cast<const uint4*>(src)[i];
+  constexpr int kAhead = 5;
+  const uint4* from = static_cast<const uint4*>(src) + threadIdx.x;
+  uint4* to = static_cast<uint4*>(dst) + threadIdx.x;
+  for (int i = threadIdx.x; i < n16; i += kAhead * kMoveThreads, from += kAhead * kMoveThreads, to += kAhead * kMoveThreads) {
+    uint4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (i + k * kMoveThreads < n16) v[k] = __ldcg(from + k * kMoveThreads);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (i + k * kMoveThreads < n16) to[k * kMoveThreads] = v[k];
+  }
 }
 // page `from` of a layer to page `to` of it, by the whole CTA
 __device__ __forceinline__ void copy_page(const PageLayer& l, int page_size, int64_t from, int64_t to) {

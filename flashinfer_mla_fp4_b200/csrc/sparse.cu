@@ -50,6 +50,7 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
   __shared__ float top_s[kWarps];
   __shared__ int most_s[2][kWarps];
   __shared__ int unsound_s;
+  __shared__ float scale_s, by_s[2];
   dependent_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int page = -1;
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
   // all of the page is asked for before anything is done with it
   constexpr int kPairs = kPage / 2, kMine = (kPairs + kSumGroups - 1) / kSumGroups, kRopeMine = (kPage + kRopeGroups - 1) / kRopeGroups;
   const int word = tid & 63, group = tid >> 6;
-  uint32_t v[kMine][2], r[kRopeMine];
+  uint32_t v[kMine][2], rw[kRopeMine];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const int pair = group + i * kSumGroups;
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
 #pragma unroll
   for (int i = 0; i < kRopeMine; ++i) {
     const int t = (tid >> 4) + i * kRopeGroups;
-    r[i] = t < kPage ? __ldcg(reinterpret_cast<const uint32_t*>(rows + t * kRowBytes + kLatent / 2) + (tid & 15)) : 0u;
+    rw[i] = t < kPage ? __ldcg(reinterpret_cast<const uint32_t*>(rows + t * kRowBytes + kLatent / 2) + (tid & 15)) : 0u;
   }
   float top = fabsf(s);
   bool unsound = !(top <= CUDART_MAX_NORMAL_F);
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
   float sum[4] = {};
 #pragma unroll
   for (int i = 0; i < kRopeMine; ++i) {
-    const float2 a = e4m3x2_to_float2(r[i] & 0xffff), b = e4m3x2_to_float2(r[i] >> 16);
+    const float2 a = e4m3x2_to_float2(rw[i] & 0xffff), b = e4m3x2_to_float2(rw[i] >> 16);
     sum[0] += a.x;
     sum[1] += a.y;
     sum[2] += b.x;
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
     lat.x += more.x;
     lat.y += more.y;
   }
-  if (tid < kRope / 2)
+  if (warp == 0)
 #pragma unroll
     for (int g = 0; g < kRopeGroups; ++g) {
       const int2 more = *reinterpret_cast<const int2*>(&rope_s[g][2 * tid]);
@@ -148,25 +149,39 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
     most_s[1][warp] = most_rope;
   }
   __syncthreads();
-  const int ml = __reduce_max_sync(0xffffffffu, most_s[0][lane & (kWarps - 1)]), mr = most_s[1][0];
-  const double of_lat = double(top) / (65534.0 * kPage), of_rope = 1.0 / (512.0 * kPage);
-  const float scale = float(fmax(double(ml) * of_lat, double(mr) * of_rope) / 127.0);
+  // One warp makes the scale and what multiplies the sums; the others wait: these are a hundred instructions of 64 bits.
+  constexpr double kLatUnit = 1.0 / (65534.0 * kPage), kRopeUnit = 1.0 / (512.0 * kPage);
+  if (warp == 0) {
+    const int ml = __reduce_max_sync(0xffffffffu, most_s[0][lane & (kWarps - 1)]), mr = most_s[1][0];
+    const float scale = float(fmax(double(ml) * (double(top) * kLatUnit), double(mr) * kRopeUnit) / 127.0);
+    const double one = 1.0 / double(scale);
+    if (lane == 0) {
+      scale_s = scale;
+      by_s[0] = float(double(top) * kLatUnit * one);
+      by_s[1] = float(kRopeUnit * one);
+    }
+  }
+  __syncthreads();
+  const float scale = scale_s;
   const bool sound = !unsound_s && scale <= CUDART_MAX_NORMAL_F, some = sound && scale > 0.f;
-  // Codes in FP32 unless that is too near the middle of two: the product is off by less than 2^-16 (three roundings of at most 127 ulp-halves).
-  const float lat32 = float(of_lat / double(scale)), rope32 = float(of_rope / double(scale));
-  auto code = [&](int sum_of, float by32, double by) -> int {
-    if (!some) return 0;
-    const float x = float(sum_of) * by32, whole = rintf(x);
+  // Codes in FP32 unless that is too near the middle of two: the product is off by less than 2^-15 (roundings of at most 127 half-ulps).
+  auto code = [&](int sum, float by, double unit) -> int {
+    const float x = float(sum) * by, whole = rintf(x);
     if (fabsf(fabsf(x - whole) - 0.5f) > 0x1p-12f && fabsf(x) < 130.f) return min(max(int(whole), -127), 127);
-    return int(fmin(fmax(rint(double(sum_of) * by / double(scale)), -127.0), 127.0));
+    return int(fmin(fmax(rint(double(sum) * unit / double(scale)), -127.0), 127.0));
   };
   char* out = reinterpret_cast<char*>(p.summary) + int64_t(page) * kQDim;
-  const int c0 = code(lat.x, lat32, of_lat), c1 = code(lat.y, lat32, of_lat);
-  *reinterpret_cast<uint16_t*>(out + dim) = uint16_t((c0 & 0xff) | (c1 & 0xff) << 8);
-  if (tid < kRope / 2) {
-    const int r0 = code(rope.x, rope32, of_rope), r1 = code(rope.y, rope32, of_rope);
-    *reinterpret_cast<uint16_t*>(out + kLatent + 2 * tid) = uint16_t((r0 & 0xff) | (r1 & 0xff) << 8);
+  int c[2] = {}, r[2] = {};
+  if (some) {
+    c[0] = code(lat.x, by_s[0], double(top) * kLatUnit);
+    c[1] = code(lat.y, by_s[0], double(top) * kLatUnit);
+    if (warp == 0) {
+      r[0] = code(rope.x, by_s[1], kRopeUnit);
+      r[1] = code(rope.y, by_s[1], kRopeUnit);
+    }
   }
+  *reinterpret_cast<uint16_t*>(out + dim) = uint16_t((c[0] & 0xff) | (c[1] & 0xff) << 8);
+  if (warp == 0) *reinterpret_cast<uint16_t*>(out + kLatent + 2 * lane) = uint16_t((r[0] & 0xff) | (r[1] & 0xff) << 8);
   if (tid == 0) p.summary_sf[page] = sound ? scale : CUDART_NAN_F;
 }
 
