@@ -199,8 +199,8 @@ def _load() -> C.CDLL:
     lib.mla_fp4_step_metadata.restype = C.c_int
     vp, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
     for name, args in {
-        "mla_fp4_summarize_pages": [vp, vp, i64, i32, vp, i64, vp, vp, vp],
-        "mla_fp4_summarize_new_pages": [vp, vp, i64, i32, vp, i64, i32, vp, i32, i32, vp, vp, vp],
+        "mla_fp4_summarize_pages": [vp, vp, i64, i32, vp, i64, vp, vp, vp, vp],
+        "mla_fp4_summarize_new_pages": [vp, vp, i64, i32, vp, i64, i32, vp, i32, i32, vp, vp, vp, vp],
         "mla_fp4_select_workspace_bytes": [i32, i32, i32, C.POINTER(C.c_size_t)],
         "mla_fp4_select_pages": [C.POINTER(SelectArgs)],
         "mla_fp4_pool_workspace_bytes": [i64, i32, i32, C.POINTER(C.c_size_t)],

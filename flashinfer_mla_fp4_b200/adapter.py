@@ -213,7 +213,7 @@ class FP4MLADecodeBackend:
         if longest != self.max_seq_len and torch.cuda.is_current_stream_capturing():  # (the graph is for other steps than this one)
             longest = self._longest_captured
         if self.sparse is not None:
-            summarize_new_pages(cache.kv_cache, cache.kv_cache_sf, cache.summary, cache.summary_sf, views[1], views[2], self.q_len)
+            summarize_new_pages(cache.kv_cache, cache.kv_cache_sf, cache.summary, cache.summary_sf, views[1], views[2], self.q_len, self.wrapper.status)
             return self._runner.run(q, cache.kv_cache, views[1], views[2], longest, self.softmax_scale, output_scale=self.output_scale,
                                     out=out, kv_cache_sf=cache.kv_cache_sf, summary=cache.summary, summary_sf=cache.summary_sf)
         return self._runner.run(q, cache.kv_cache, views[1], views[2], longest, self.softmax_scale,

@@ -11,7 +11,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = Path(os.environ.get("MLA_FP4_B200_LIB") or (PKG_DIR / "libmla_fp4_b200.so"))
-SOURCES = ["abi.cu", "kernels_simt.cu", "combine.cu", "cache_write.cu", "cp_exchange.cu", "sparse.cu", "score_sm100.cu", "pages.cu", "decode_sm100.cu"]
+SOURCES = ["abi.cu", "kernels_simt.cu", "combine.cu", "cache_write.cu", "cp_exchange.cu", "sparse.cu", "score_sm100.cu", "summarize_sm100.cu", "pages.cu", "decode_sm100.cu"]
 NATIVE_PATH = PKG_DIR / "_native.so"
 NATIVE_SOURCE = CSRC / "py_native.cpp"
 HEADERS = ["common.cuh", "decode_pair.cuh", "dequant.cuh", "launch.h", "ptx_sm100.cuh", "sparse.cuh", "../../include/mla_fp4_b200.h"]

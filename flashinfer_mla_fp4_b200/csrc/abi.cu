@@ -470,13 +470,17 @@ int mla_fp4_step_metadata(const int32_t* block_tables, int64_t block_table_strid
 }
 
 namespace {
-int summarize(mla::SummarizeParams& p, int64_t ctas, void* stream) {
+int summarize(mla::SummarizeParams& p, int64_t ctas, int32_t* status, void* stream) {
   if (!page_size_ok(p.page_size)) return fail(MLA_FP4_ERR_UNSUPPORTED, "page_size must be one of 8, 16, 32, 64, 128");
   if (p.num_pages <= 0 || p.num_pages > INT_MAX) return fail(MLA_FP4_ERR_BAD_ARG, "num_pages out of range");
   if (!p.kv_cache || !p.kv_cache_sf || !p.summary || !p.summary_sf) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
   if (reinterpret_cast<uintptr_t>(p.kv_cache) % 16 || reinterpret_cast<uintptr_t>(p.summary) % 16) return fail(MLA_FP4_ERR_BAD_ARG, "kv_cache and summary must be 16-byte aligned");
   if (ctas > INT_MAX) return fail(MLA_FP4_ERR_UNSUPPORTED, "too many pages in one call");
-  cudaError_t e = mla::launch_summarize(p, ctas, reinterpret_cast<cudaStream_t>(stream));
+  p.status = status;
+  p.wait_polls = 1u << 22;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  cudaError_t e = mla::launch_summarize(p, ctas, sms, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(MLA_FP4_ERR_CUDA, std::string("summarize launch: ") + cudaGetErrorString(e));
   return MLA_FP4_OK;
 }
@@ -487,7 +491,7 @@ int table_cap(int width, int page_size) { return std::min(seq_cap_of(width, page
 }  // namespace
 
 int mla_fp4_summarize_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
-                            const int32_t* page_ids, int64_t count, void* summary, float* summary_sf, void* stream) {
+                            const int32_t* page_ids, int64_t count, void* summary, float* summary_sf, int32_t* status, void* stream) {
   if (count < 0) return fail(MLA_FP4_ERR_BAD_ARG, "count out of range");
   if (count == 0) return MLA_FP4_OK;
   if (!page_ids) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
@@ -495,13 +499,13 @@ int mla_fp4_summarize_pages(const void* kv_cache, const float* kv_cache_sf, int6
   p.kv_cache = static_cast<const uint8_t*>(kv_cache); p.kv_cache_sf = kv_cache_sf;
   p.summary = static_cast<int8_t*>(summary); p.summary_sf = summary_sf;
   p.page_ids = page_ids; p.num_pages = num_pages; p.page_size = page_size;
-  return summarize(p, count, stream);
+  return summarize(p, count, status, stream);
 }
 
 int mla_fp4_summarize_new_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
                                 const int32_t* block_tables, int64_t block_table_stride, int32_t width,
                                 const int32_t* seq_lens, int32_t batch, int32_t new_tokens, void* summary,
-                                float* summary_sf, void* stream) {
+                                float* summary_sf, int32_t* status, void* stream) {
   if (batch < 0 || width < 0 || new_tokens < 0) return fail(MLA_FP4_ERR_BAD_ARG, "batch/width/new_tokens out of range");
   if (batch == 0 || width == 0 || new_tokens == 0) return MLA_FP4_OK;
   if (!block_tables || !seq_lens) return fail(MLA_FP4_ERR_BAD_ARG, "null pointer");
@@ -513,7 +517,7 @@ int mla_fp4_summarize_new_pages(const void* kv_cache, const float* kv_cache_sf, 
   p.num_pages = num_pages; p.page_size = page_size; p.new_tokens = new_tokens;
   p.per_request = std::min(width, int32_t((int64_t(new_tokens) + page_size - 1) / page_size));
   p.seq_cap = table_cap(width, page_size);
-  return summarize(p, int64_t(batch) * p.per_request, stream);
+  return summarize(p, int64_t(batch) * p.per_request, status, stream);
 }
 
 int mla_fp4_select_workspace_bytes(int32_t batch, int32_t q_len, int32_t width, size_t* bytes_out) {

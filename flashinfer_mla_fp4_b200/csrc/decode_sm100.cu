@@ -1853,21 +1853,34 @@ bool encode_q_maps(const DecodeParams& p, CUtensorMap* lat, CUtensorMap* rope) {
   return encode_map(lat, p.q, 4, dims, strides, box_lat, CU_TENSOR_MAP_SWIZZLE_128B) &&
          encode_map(rope, p.q, 4, dims, strides, box_rope, CU_TENSOR_MAP_SWIZZLE_64B);
 }
-// the RoPE bytes of a page, and the cache as 4-bit elements: 640 per row (the 512 latent codes, then the RoPE bytes seen as
-// nibbles and never fetched through this map), page_size rows per page; a box is one 128-dim block of `rows` rows of a page
-bool encode_kv_maps(const DecodeParams& p, uint32_t rows, CUtensorMap* lat, CUtensorMap* rope) {
-  const uint64_t dims[3] = {uint64_t(kRowBytes), uint64_t(p.page_size), uint64_t(p.num_pages)};
-  const uint64_t strides[2] = {uint64_t(kRowBytes), uint64_t(kRowBytes) * uint64_t(p.page_size)};
-  const uint32_t box[3] = {64, rows, 1};
-  if (!encode_map(rope, p.kv_cache, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) return false;
+}  // namespace
+
+// The cache as 4-bit elements: 640 per row (the 512 latent codes, then the RoPE bytes seen as nibbles and never fetched through this map), page_size
+// rows per page; a box is one 128-dim block of `rows` rows of a page
+bool encode_latent_map(const void* kv_cache, int64_t num_pages, int32_t page_size, uint32_t rows, CUtensorMap* map) {
   EncodeTiledFn fn = get_encode_fn();
-  cuuint64_t gd[3] = {cuuint64_t(2 * kRowBytes), cuuint64_t(p.page_size), cuuint64_t(p.num_pages)};
-  cuuint64_t gs[2] = {cuuint64_t(kRowBytes), cuuint64_t(kRowBytes) * cuuint64_t(p.page_size)};
+  if (!fn) return false;
+  cuuint64_t gd[3] = {cuuint64_t(2 * kRowBytes), cuuint64_t(page_size), cuuint64_t(num_pages)};
+  cuuint64_t gs[2] = {cuuint64_t(kRowBytes), cuuint64_t(kRowBytes) * cuuint64_t(page_size)};
   cuuint32_t bx[3] = {128, cuuint32_t(rows), 1};
   cuuint32_t es[3] = {1, 1, 1};
-  return fn(lat, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, const_cast<void*>(p.kv_cache), gd, gs, bx, es,
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 3, const_cast<void*>(kv_cache), gd, gs, bx, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool encode_rope_map(const void* kv_cache, int64_t num_pages, int32_t page_size, uint32_t rows, bool swizzled, CUtensorMap* map) {
+  const uint64_t dims[3] = {uint64_t(kRowBytes), uint64_t(page_size), uint64_t(num_pages)};
+  const uint64_t strides[2] = {uint64_t(kRowBytes), uint64_t(kRowBytes) * uint64_t(page_size)};
+  const uint32_t box[3] = {64, rows, 1};
+  return encode_map(map, kv_cache, 3, dims, strides, box, swizzled ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+namespace {
+
+bool encode_kv_maps(const DecodeParams& p, uint32_t rows, CUtensorMap* lat, CUtensorMap* rope) {
+  return encode_rope_map(p.kv_cache, p.num_pages, p.page_size, rows, true, rope) &&
+         encode_latent_map(p.kv_cache, p.num_pages, p.page_size, rows, lat);
 }
 
 }  // namespace

@@ -1,5 +1,6 @@
 // Kernel parameter blocks and launcher prototypes shared by the translation units.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -110,8 +111,15 @@ struct SummarizeParams {
   int64_t block_table_stride, num_pages;
   int32_t page_size, per_request, new_tokens;
   int32_t seq_cap;  // as in DecodeParams
+  uint32_t wait_polls;
+  int32_t* status;
 };
-cudaError_t launch_summarize(const SummarizeParams& p, int64_t ctas, cudaStream_t stream);
+cudaError_t launch_summarize(const SummarizeParams& p, int64_t count, int sms, cudaStream_t stream);
+cudaError_t launch_summarize_many(const SummarizeParams& p, int64_t count, int sms, cudaStream_t stream);  // summarize_sm100.cu
+// decode_sm100.cu: the cache as 4-bit elements, a box being one 128-dim block of `rows` rows of a page, in the MMA's form
+bool encode_latent_map(const void* kv_cache, int64_t num_pages, int32_t page_size, uint32_t rows, CUtensorMap* map);
+// the RoPE bytes of `rows` rows of a page, as they are or with the 64-byte swizzle
+bool encode_rope_map(const void* kv_cache, int64_t num_pages, int32_t page_size, uint32_t rows, bool swizzled, CUtensorMap* map);
 struct SelectParams {
   const uint8_t* q;
   int64_t q_stride_batch, q_stride_qpos, q_stride_head;

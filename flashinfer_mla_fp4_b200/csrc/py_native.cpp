@@ -380,11 +380,11 @@ bool query_ok(const at::Tensor& q) {
   return q.is_cuda() && q.dim() == 4 && q.scalar_type() == at::kFloat8_e4m3fn && q.size(3) == MLA_FP4_LATENT_DIM + MLA_FP4_ROPE_DIM && q.stride(3) == 1 &&
          q.size(0) > 0 && q.size(1) > 0 && q.size(2) > 0 && q.size(2) <= 128;
 }
-// summarize(kv_cache, kv_cache_sf, summary, summary_sf, page_ids, block_tables, seq_lens, new_tokens) -> whether it was launched; page_ids, or
+// summarize(kv_cache, kv_cache_sf, summary, summary_sf, page_ids, block_tables, seq_lens, new_tokens, status or None) -> whether it was launched; page_ids, or
 // the other three
 PyObject* summarize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 8) return PyErr_Format(PyExc_TypeError, "summarize takes 8 arguments");
+  if (n != 9) return PyErr_Format(PyExc_TypeError, "summarize takes 9 arguments");
   const at::Tensor *kv = tensor(a[0]), *sf = tensor(a[1]), *su = tensor(a[2]), *ssf = tensor(a[3]);
   if (!kv || !sf || !su || !ssf || !cache_ok(*kv, *sf)) Py_RETURN_FALSE;
   const at::Device dev = kv->device();
@@ -401,6 +401,9 @@ PyObject* summarize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     sl = tensor(a[6]);
     if (!bt || !sl || !integer(a[7], &fresh) || fresh < 0 || fresh > INT32_MAX || !tables_ok(*bt, *sl, dev)) Py_RETURN_FALSE;
   }
+  const at::Tensor* st = a[8] == Py_None ? nullptr : tensor(a[8]);
+  if (a[8] != Py_None && (!st || !plain(*st, at::kInt, {8}, dev))) Py_RETURN_FALSE;
+  int32_t* status = st ? static_cast<int32_t*>(st->data_ptr()) : nullptr;
   c10::cuda::CUDAGuard guard(dev);
   const void* kv_p = kv->data_ptr();
   const float* sf_p = static_cast<const float*>(sf->data_ptr());
@@ -410,9 +413,9 @@ PyObject* summarize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int rc;
   {
     NoGil released;
-    rc = by_id ? abi.summarize_pages(kv_p, sf_p, pages, int32_t(page), static_cast<const int32_t*>(ids->data_ptr()), ids->numel(), su_p, ssf_p, stream)
+    rc = by_id ? abi.summarize_pages(kv_p, sf_p, pages, int32_t(page), static_cast<const int32_t*>(ids->data_ptr()), ids->numel(), su_p, ssf_p, status, stream)
                : abi.summarize_new_pages(kv_p, sf_p, pages, int32_t(page), static_cast<const int32_t*>(bt->data_ptr()), bt->stride(0), int32_t(bt->size(1)),
-                                         static_cast<const int32_t*>(sl->data_ptr()), int32_t(bt->size(0)), int32_t(fresh), su_p, ssf_p, stream);
+                                         static_cast<const int32_t*>(sl->data_ptr()), int32_t(bt->size(0)), int32_t(fresh), su_p, ssf_p, status, stream);
   }
   if (rc != MLA_FP4_OK) return raise_status(rc);
   Py_RETURN_TRUE;

@@ -55,13 +55,7 @@ __device__ __forceinline__ bool wait(const Ctx& c, const unsigned long long& b, 
     if (c.s.abort) return false;
   }
   c.s.abort = 1;
-  if (c.p.status) {
-    c.p.status[1] = int(bar(b));
-    c.p.status[2] = blockIdx.x;
-    c.p.status[3] = threadIdx.x;
-    c.p.status[4] = int(parity);
-    c.p.status[0] = MLA_FP4_ERR_DEVICE_TIMEOUT;
-  }
+  report_timeout(c.p.status, bar(b), parity);
   return false;
 }
 

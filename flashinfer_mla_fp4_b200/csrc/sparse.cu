@@ -53,15 +53,8 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
   __shared__ float scale_s, by_s[2];
   dependent_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int page = -1;
-  if (p.page_ids) {
-    page = __ldcg(p.page_ids + blockIdx.x);
-  } else {  // the pages that the last new_tokens positions of a request have filled, the newest first
-    const int b = blockIdx.x / p.per_request, j = blockIdx.x - b * p.per_request;
-    const int len = min(__ldcg(p.seq_lens + b), p.seq_cap), at = len / kPage - 1 - j;
-    if (at >= 0 && (at + 1) * int64_t(kPage) > int64_t(len) - p.new_tokens) page = __ldcg(p.block_tables + int64_t(b) * p.block_table_stride + at);
-  }
-  if (page < 0 || page >= p.num_pages) return;
+  const int page = page_of_item<kPage>(p, blockIdx.x);
+  if (page < 0) return;
   const uint8_t* rows = p.kv_cache + int64_t(page) * kPage * kRowBytes;
   const float s = tid < kPage ? __ldcg(p.kv_cache_sf + int64_t(page) * kPage + tid) : 0.f;
   // all of the page is asked for before anything is done with it
@@ -149,40 +142,27 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
     most_s[1][warp] = most_rope;
   }
   __syncthreads();
-  // One warp makes the scale and what multiplies the sums; the others wait: these are a hundred instructions of 64 bits.
+  // One warp makes the scale and what multiplies the sums; the others wait.
   constexpr double kLatUnit = 1.0 / (65534.0 * kPage), kRopeUnit = 1.0 / (512.0 * kPage);
   if (warp == 0) {
     const int ml = __reduce_max_sync(0xffffffffu, most_s[0][lane & (kWarps - 1)]), mr = most_s[1][0];
-    const float scale = float(fmax(double(ml) * (double(top) * kLatUnit), double(mr) * kRopeUnit) / 127.0);
-    const double one = 1.0 / double(scale);
+    const float scale = unsound_s ? CUDART_NAN_F : summary_scale(ml, mr, top, kLatUnit, kRopeUnit);
     if (lane == 0) {
       scale_s = scale;
-      by_s[0] = float(double(top) * kLatUnit * one);
-      by_s[1] = float(kRopeUnit * one);
+      by_s[0] = top / scale * float(kLatUnit);
+      by_s[1] = float(kRopeUnit) / scale;
     }
   }
   __syncthreads();
   const float scale = scale_s;
-  const bool sound = !unsound_s && scale <= CUDART_MAX_NORMAL_F, some = sound && scale > 0.f;
-  // Codes in FP32 unless that is too near the middle of two: the product is off by less than 2^-15 (roundings of at most 127 half-ulps).
-  auto code = [&](int sum, float by, double unit) -> int {
-    const float x = float(sum) * by, whole = rintf(x);
-    if (fabsf(fabsf(x - whole) - 0.5f) > 0x1p-12f && fabsf(x) < 130.f) return min(max(int(whole), -127), 127);
-    return int(fmin(fmax(rint(double(sum) * unit / double(scale)), -127.0), 127.0));
-  };
   char* out = reinterpret_cast<char*>(p.summary) + int64_t(page) * kQDim;
-  int c[2] = {}, r[2] = {};
-  if (some) {
-    c[0] = code(lat.x, by_s[0], double(top) * kLatUnit);
-    c[1] = code(lat.y, by_s[0], double(top) * kLatUnit);
-    if (warp == 0) {
-      r[0] = code(rope.x, by_s[1], kRopeUnit);
-      r[1] = code(rope.y, by_s[1], kRopeUnit);
-    }
-  }
+  const int c[2] = {summary_code(lat.x, scale, by_s[0], top, kLatUnit), summary_code(lat.y, scale, by_s[0], top, kLatUnit)};
   *reinterpret_cast<uint16_t*>(out + dim) = uint16_t((c[0] & 0xff) | (c[1] & 0xff) << 8);
-  if (warp == 0) *reinterpret_cast<uint16_t*>(out + kLatent + 2 * lane) = uint16_t((r[0] & 0xff) | (r[1] & 0xff) << 8);
-  if (tid == 0) p.summary_sf[page] = sound ? scale : CUDART_NAN_F;
+  if (warp == 0) {
+    const int r[2] = {summary_code(rope.x, scale, by_s[1], 1.f, kRopeUnit), summary_code(rope.y, scale, by_s[1], 1.f, kRopeUnit)};
+    *reinterpret_cast<uint16_t*>(out + kLatent + 2 * lane) = uint16_t((r[0] & 0xff) | (r[1] & 0xff) << 8);
+  }
+  if (tid == 0) p.summary_sf[page] = scale;
 }
 
 // ------------------------------------------------------------------------------------------ selection
@@ -337,10 +317,17 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
 
 }  // namespace
 
-cudaError_t launch_summarize(const SummarizeParams& p, int64_t ctas, cudaStream_t stream) {
+// From how many tokens on pages go to summarize_many_kernel, this kernel -> that one, us: pages of 64 tokens, 76000 tokens 11.1 -> 11.8, 150000
+// 18.3 -> 16.6, 300000 32.6 -> 26.3; of 32, 12.4 -> 13.9, 21.3 -> 19.5, 39.6 -> 32.5; of 128, 11.0 -> 11.2, 17.0 -> 15.6, 28.2 -> 24.2.  Pages of 16
+// tokens, eight to a tile, took longer there whatever their number (300000 tokens 64.3 -> 73.4), and so did those of 8 (116.4 -> 120.3).
+constexpr int64_t kManyTokens = 131072;
+constexpr int kManyPage = 32;
+
+cudaError_t launch_summarize(const SummarizeParams& p, int64_t count, int sms, cudaStream_t stream) {
+  if (p.page_size >= kManyPage && count * p.page_size >= kManyTokens && reinterpret_cast<uintptr_t>(p.kv_cache) % 32 == 0) return launch_summarize_many(p, count, sms, stream);
   const auto kernel = p.page_size == 8 ? summarize_kernel<8> : p.page_size == 16 ? summarize_kernel<16> : p.page_size == 32 ? summarize_kernel<32>
                       : p.page_size == 64 ? summarize_kernel<64> : summarize_kernel<128>;
-  return launch_dependent(kernel, dim3(unsigned(ctas)), kSumThreads, 0, stream, p);
+  return launch_dependent(kernel, dim3(unsigned(count)), kSumThreads, 0, stream, p);
 }
 
 cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream) {

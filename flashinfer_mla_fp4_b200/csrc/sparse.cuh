@@ -57,4 +57,56 @@ __device__ __forceinline__ uint32_t key_of(float score) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+
+// The page of an item of a summary call, -1 where there is none: of the list, or the j-th newest of the pages that the last new_tokens positions of
+// a request have filled.
+template <int kPage>
+__device__ __forceinline__ int page_of_item(const SummarizeParams& p, int64_t item) {
+  int page = -1;
+  if (p.page_ids) {
+    page = __ldcg(p.page_ids + item);
+  } else {
+    const int b = int(item / p.per_request), j = int(item - int64_t(b) * p.per_request);
+    const int len = min(__ldcg(p.seq_lens + b), p.seq_cap), at = len / kPage - 1 - j;
+    if (at >= 0 && (at + 1) * int64_t(kPage) > int64_t(len) - p.new_tokens) page = __ldcg(p.block_tables + int64_t(b) * p.block_table_stride + at);
+  }
+  return page >= 0 && page < p.num_pages ? page : -1;
+}
+// The scale of a summary, max(most_lat * top * lat_unit, most_rope * rope_unit) / 127 to the nearest FP32 value; NaN where that is not finite.  A quotient
+// in FP32, and the exact remainder in 64 bits says whether a neighbour is nearer (a division in 64 bits is several hundred clk;
+// a quotient half-way between two FP32 values has more bits than these sums give it).
+__device__ __forceinline__ float summary_scale(int most_lat, int most_rope, float top, double lat_unit, double rope_unit) {
+  const double largest = fmax(double(most_lat) * (double(top) * lat_unit), double(most_rope) * rope_unit);
+  const float q = __double2float_rn(largest * (1.0 / 127.0));
+  if (!(q < 3e38f)) return __uint_as_float(0x7fffffffu);
+  if (q < 1e-30f) return float(largest / 127.0);  // (where an ulp is not a fixed part of the value)
+  const float up = __uint_as_float(__float_as_uint(q) + 1), down = __uint_as_float(__float_as_uint(q) - 1);
+  const double off = fma(-127.0, double(q), largest);  // q is the nearest but for the rounding of the product
+  return off > 63.5 * double(up - q) ? up : off < -63.5 * double(q - down) ? down : q;
+}
+// round(sum * top * unit / scale), within [-127, 127]; 0 where the scale is 0 or NaN.  `by` is top * unit / scale in FP32, and will do unless the
+// product is too near the middle of two whole numbers (it is off by less than 2^-14: roundings of 5 * 127 half-ulps of 1): then the
+// sum is compared with the middle in 64 bits.
+__device__ __forceinline__ int summary_code(int sum, float scale, float by, float top, double unit) {
+  const float x = float(sum) * by;
+  float whole = rintf(x);
+  const float middle = truncf(x) + copysignf(0.5f, x);
+  if (!(fabsf(x - middle) > 0x1p-14f)) {
+    const double over = fma(double(-middle), double(scale), double(sum) * (double(top) * unit));  // of the middle, times the scale
+    const float toward = copysignf(0.5f, x);
+    whole = over == 0.0 ? rintf(middle) : (over > 0.0) == (x > 0.f) ? middle + toward : middle - toward;
+  }
+  return scale > 0.f ? int(fminf(fmaxf(whole, -127.f), 127.f)) : 0;
+}
+
+// what a bounded wait that ran out leaves in the status words
+__device__ __forceinline__ void report_timeout(int32_t* status, uint32_t bar, uint32_t parity) {
+  if (!status) return;
+  status[1] = int(bar);
+  status[2] = blockIdx.x;
+  status[3] = threadIdx.x;
+  status[4] = int(parity);
+  status[0] = MLA_FP4_ERR_DEVICE_TIMEOUT;
+}
+
 }  // namespace mla

@@ -91,33 +91,36 @@ def check_summary(summary, summary_sf, pages: Optional[int], device) -> int:
 
 @api_logged
 def summarize_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tensor,
-                    page_ids: torch.Tensor) -> None:
+                    page_ids: torch.Tensor, status: Optional[torch.Tensor] = None) -> None:
     """Write the summaries of full pages: ``summary`` int8 [pages, 576] and ``summary_sf`` f32 [pages], at the numbers in ``page_ids``
     (int32, contiguous, on the device; those outside the pool are skipped, one that is named twice is written twice alike).
 
-    All ``page_size`` rows of a page enter its summary, so call it for pages that are full.  Asynchronous on the current stream."""
-    if _native.summarize(kv_cache, kv_cache_sf, summary, summary_sf, page_ids, None, None, 0):
+    All ``page_size`` rows of a page enter its summary, so call it for pages that are full.  ``status`` (int32 [8], zeroed) gets the error of a
+    device-side wait that ran out.  Asynchronous on the current stream."""
+    if _native.summarize(kv_cache, kv_cache_sf, summary, summary_sf, page_ids, None, None, 0, status):
         return  # the common form, checked and launched natively; otherwise nothing was done
     pages, page_size = check_cache(kv_cache, kv_cache_sf)
     dev = kv_cache.device
     check_summary(summary, summary_sf, pages, dev)
     check_tensor("page_ids", page_ids, torch.int32, (None,), dev)
+    if status is not None:
+        check_tensor("status", status, torch.int32, (8,), dev)
     if page_ids.numel() == 0:
         return
     with torch.cuda.device(dev):
         _cabi.check(_cabi.lib.mla_fp4_summarize_pages(kv_cache.data_ptr(), kv_cache_sf.data_ptr(), pages, page_size, page_ids.data_ptr(),
                                                       page_ids.numel(), summary.data_ptr(), summary_sf.data_ptr(),
-                                                      torch.cuda.current_stream(dev).cuda_stream))
+                                                      None if status is None else status.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
 
 
 @api_logged
 def summarize_new_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tensor,
-                        block_tables: torch.Tensor, seq_lens: torch.Tensor, new_tokens: int) -> None:
+                        block_tables: torch.Tensor, seq_lens: torch.Tensor, new_tokens: int, status: Optional[torch.Tensor] = None) -> None:
     """Write the summaries of the pages that the newest ``new_tokens`` tokens of each request have filled.
 
     ``seq_lens`` (int32 [batch]) counts the new tokens, ``block_tables`` int32 [batch, max_pages].  What a step calls behind
     ``write_tokens``; a page that the step has not filled is left alone.  Asynchronous on the current stream."""
-    if _native.summarize(kv_cache, kv_cache_sf, summary, summary_sf, None, block_tables, seq_lens, new_tokens):
+    if _native.summarize(kv_cache, kv_cache_sf, summary, summary_sf, None, block_tables, seq_lens, new_tokens, status):
         return
     pages, page_size = check_cache(kv_cache, kv_cache_sf)
     dev = kv_cache.device
@@ -125,6 +128,8 @@ def summarize_new_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summa
     check_tables(block_tables, seq_lens, dev)
     if new_tokens < 0:
         raise ValueError(f"new_tokens must not be negative, got {new_tokens}")
+    if status is not None:
+        check_tensor("status", status, torch.int32, (8,), dev)
     batch, width = block_tables.shape
     if batch == 0 or width == 0 or new_tokens == 0:
         return
@@ -132,7 +137,7 @@ def summarize_new_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summa
         _cabi.check(_cabi.lib.mla_fp4_summarize_new_pages(
             kv_cache.data_ptr(), kv_cache_sf.data_ptr(), pages, page_size, block_tables.data_ptr(), block_tables.stride(0), width,
             seq_lens.data_ptr(), batch, min(int(new_tokens), 2**31 - 1), summary.data_ptr(), summary_sf.data_ptr(),
-            torch.cuda.current_stream(dev).cuda_stream))
+            None if status is None else status.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
 
 
 @api_logged
@@ -296,6 +301,11 @@ class BatchMLASparseDecodeFP4Wrapper:
         scores = _aligned(lens_end)
         part = self._workspace_buffer[at:lens_end].view(torch.int32)
         return part[:rows * budget].view(rows, budget), part[rows * budget:], self._workspace_buffer[scores:need]
+
+    @property
+    def status(self) -> Optional[torch.Tensor]:
+        """The device status words (int32 [8]), for ``summarize_new_pages`` to report in too."""
+        return self._dense._status
 
     def device_status(self) -> Tuple[int, ...]:
         return self._dense.device_status()

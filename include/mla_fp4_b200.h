@@ -284,13 +284,14 @@ int mla_fp4_step_metadata(const int32_t* block_tables, int64_t block_table_strid
      mla_fp4_summarize_pages: of page_ids int32 [count]; ids outside the pool are skipped.
      mla_fp4_summarize_new_pages: of the pages that the last new_tokens positions of each request have filled (seq_lens counts them):
        what a step calls behind mla_fp4_cache_write.  width is that of a block-table row in pages.
-   Asynchronous on `stream`, nothing allocated. */
+   Asynchronous on `stream`, nothing allocated.  status as in MlaFp4DecodeArgs, may be NULL. */
 int mla_fp4_summarize_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
-                            const int32_t* page_ids, int64_t count, void* summary, float* summary_sf, void* stream);
+                            const int32_t* page_ids, int64_t count, void* summary, float* summary_sf, int32_t* status,
+                            void* stream);
 int mla_fp4_summarize_new_pages(const void* kv_cache, const float* kv_cache_sf, int64_t num_pages, int32_t page_size,
                                 const int32_t* block_tables, int64_t block_table_stride, int32_t width,
                                 const int32_t* seq_lens, int32_t batch, int32_t new_tokens, void* summary,
-                                float* summary_sf, void* stream);
+                                float* summary_sf, int32_t* status, void* stream);
 
 /* Selection: for every query position (row = request * q_len + position) the pages it attends to, as a block table int32
    [rows][budget] and lengths int32 [rows] for mla_fp4_decode with batch = rows, q_len = 1.  Of a request with no more than

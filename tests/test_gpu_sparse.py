@@ -94,6 +94,53 @@ def test_summaries_of_the_pages_that_a_step_has_filled(page, new):
     assert torch.equal(summary.cpu(), want) and torch.equal(ssf.cpu(), want_sf)
 
 
+@pytest.mark.parametrize("page", [32, 64, 128])
+def test_summaries_of_many_pages(page):
+    """Enough pages for the kernel that has the sums made by the tensor cores: the bytes that the other one writes, page for page, and the oracle's
+    for some; outlying pages among them, pages that are not named, an odd number of them, a last tile that is not full."""
+    dev = _dev()
+    from flashinfer_mla_fp4_b200.sparse import summarize_pages
+
+    few = 24
+    kv, sf = _pages(few, page, page + 1)
+    sf[1], sf[2, 3], sf[3, 0] = 0.0, float("inf"), float("nan")
+    kv[4, page - 1, 300], kv[5, 0, 256] = 0x7F, 0xFF
+    sf[6, ::2] *= -1
+    sf[7] *= 1e-38
+    sf[8], kv[8, :, 256:] = 1e-45, 0
+    sf[9], kv[9, :, :256] = 3e38, 0x77
+    sf[10, 1:] = sf[10, 0] * 1e-6
+    kv[11] = 0
+    kv[12, :, 256:] = 0x7E
+    kv[13, :, :256], sf[13] = 0xFF, 1.0
+    want, want_sf = _oracle_summaries(kv, sf)
+    pool = 140000 // page + 3
+    g = torch.Generator(device=dev).manual_seed(page)
+    which = torch.randint(0, few, (pool,), generator=g, device=dev)
+    kv_all, sf_all = kv.to(dev)[which], sf.to(dev)[which]
+    ids = torch.randperm(pool, generator=g, device=dev).int()[: pool - 5]
+    ids = torch.cat((ids, torch.tensor([-1, pool, 2**31 - 1], dtype=torch.int32, device=dev), ids[:1]))
+    ids = ids[torch.randperm(ids.numel(), generator=g, device=dev)].contiguous()
+    assert ids.numel() * page >= 131072
+    summary, ssf = torch.full((pool, 576), 9, dtype=torch.int8, device=dev), torch.full((pool,), 9.0, device=dev)
+    status = torch.zeros(8, dtype=torch.int32, device=dev)
+    summarize_pages(kv_all, sf_all, summary, ssf, ids, status)
+    named = torch.zeros(pool, dtype=torch.bool, device=dev)
+    named[ids[(ids >= 0) & (ids < pool)].long()] = True
+    exp, exp_sf = want.to(dev)[which], want_sf.to(dev)[which]
+    exp[~named], exp_sf[~named] = 9, 9.0
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0
+    assert torch.equal(summary, exp) and _same(ssf, exp_sf)
+    # a cache that starts on 16 bytes but not on 32 goes to the other kernel
+    raw = torch.empty(kv_all.numel() + 64, dtype=torch.uint8, device=dev)
+    start = (16 - raw.data_ptr()) % 32
+    odd = raw[start:start + kv_all.numel()].view_as(kv_all).copy_(kv_all)
+    again, again_sf = torch.full_like(summary, 9), torch.full_like(ssf, 9.0)
+    summarize_pages(odd, sf_all, again, again_sf, ids)
+    assert torch.equal(again, exp) and _same(again_sf, exp_sf)
+
+
 def _selection_case(lens, heads, page, q_len, seed, odd=False):
     g = torch.Generator().manual_seed(seed)
     used = [max(0, -(-n // page)) for n in lens]

@@ -75,14 +75,14 @@ def test_abi_refuses_before_any_launch():
                      (dict(summary=P + 4), bad), (dict(workspace_bytes=31), _cabi.ERR_WORKSPACE_TOO_SMALL),
                      (dict(workspace=None), _cabi.ERR_WORKSPACE_TOO_SMALL), (dict(batch=0), _cabi.OK)):
         assert args_of(**kw) == code, (kw, _cabi.last_error())
-    assert lib.mla_fp4_summarize_pages(P, P, 4, 24, P, 1, P, P, None) == _cabi.ERR_UNSUPPORTED
-    assert lib.mla_fp4_summarize_pages(P, P, 0, 16, P, 1, P, P, None) == bad
-    assert lib.mla_fp4_summarize_pages(P + 4, P, 4, 16, P, 1, P, P, None) == bad
-    assert lib.mla_fp4_summarize_pages(P, P, 4, 16, None, 1, P, P, None) == bad
-    assert lib.mla_fp4_summarize_pages(P, P, 4, 16, None, 0, P, P, None) == _cabi.OK
-    assert lib.mla_fp4_summarize_new_pages(P, P, 4, 16, P, 4, 4, P, 1, -1, P, P, None) == bad
-    assert lib.mla_fp4_summarize_new_pages(P, P, 4, 16, None, 4, 4, P, 1, 1, P, P, None) == bad
-    assert lib.mla_fp4_summarize_new_pages(P, P, 4, 16, P, 4, 4, P, 0, 1, P, P, None) == _cabi.OK
+    assert lib.mla_fp4_summarize_pages(P, P, 4, 24, P, 1, P, P, None, None) == _cabi.ERR_UNSUPPORTED
+    assert lib.mla_fp4_summarize_pages(P, P, 0, 16, P, 1, P, P, None, None) == bad
+    assert lib.mla_fp4_summarize_pages(P + 4, P, 4, 16, P, 1, P, P, None, None) == bad
+    assert lib.mla_fp4_summarize_pages(P, P, 4, 16, None, 1, P, P, None, None) == bad
+    assert lib.mla_fp4_summarize_pages(P, P, 4, 16, None, 0, P, P, None, None) == _cabi.OK
+    assert lib.mla_fp4_summarize_new_pages(P, P, 4, 16, P, 4, 4, P, 1, -1, P, P, None, None) == bad
+    assert lib.mla_fp4_summarize_new_pages(P, P, 4, 16, None, 4, 4, P, 1, 1, P, P, None, None) == bad
+    assert lib.mla_fp4_summarize_new_pages(P, P, 4, 16, P, 4, 4, P, 0, 1, P, P, None, None) == _cabi.OK
     layer = (_cabi.PageLayer * 1)()
     layer[0].kv_cache, layer[0].kv_cache_sf = P, P
     assert lib.mla_fp4_copy_pages(layer, 0, 4, 16, P, P, 1, None) == bad
