@@ -20,7 +20,7 @@ namespace mla {
 namespace {
 
 // ------------------------------------------------------------------------------------------ summaries
-// A CTA per page.  Latent: a thread has eight dims (a 32-bit word of a row) of every fourth pair of tokens; two tokens at a time, their values as
+// A CTA per page of 32 tokens or more.  Latent: a thread has eight dims (a 32-bit word of a row) of every fourth pair of tokens; two tokens at a time, their values as
 // signed bytes side by side, go through dp2a with the two 16-bit weights.  RoPE: a thread has four dims of every sixteenth token; sums of eight
 // values of at most 448 in steps of 2^-9 are exact in FP32, and whole numbers of 2^-9 from there on.
 constexpr int kSumThreads = 256, kSumGroups = kSumThreads / 64, kRopeGroups = kSumThreads / 16;
@@ -58,19 +58,19 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
   const uint8_t* rows = p.kv_cache + int64_t(page) * kPage * kRowBytes;
   const float s = tid < kPage ? __ldcg(p.kv_cache_sf + int64_t(page) * kPage + tid) : 0.f;
   // all of the page is asked for before anything is done with it
-  constexpr int kPairs = kPage / 2, kMine = (kPairs + kSumGroups - 1) / kSumGroups, kRopeMine = (kPage + kRopeGroups - 1) / kRopeGroups;
+  constexpr int kMine = kPage / 2 / kSumGroups, kRopeMine = kPage / kRopeGroups;
   const int word = tid & 63, group = tid >> 6;
   uint32_t v[kMine][2], rw[kRopeMine];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const int pair = group + i * kSumGroups;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) v[i][k] = pair < kPairs ? __ldcg(reinterpret_cast<const uint32_t*>(rows + (2 * pair + k) * kRowBytes) + word) : 0u;
+    for (int k = 0; k < 2; ++k) v[i][k] = __ldcg(reinterpret_cast<const uint32_t*>(rows + (2 * pair + k) * kRowBytes) + word);
   }
 #pragma unroll
   for (int i = 0; i < kRopeMine; ++i) {
     const int t = (tid >> 4) + i * kRopeGroups;
-    rw[i] = t < kPage ? __ldcg(reinterpret_cast<const uint32_t*>(rows + t * kRowBytes + kLatent / 2) + (tid & 15)) : 0u;
+    rw[i] = __ldcg(reinterpret_cast<const uint32_t*>(rows + t * kRowBytes + kLatent / 2) + (tid & 15));
   }
   float top = fabsf(s);
   bool unsound = !(top <= CUDART_MAX_NORMAL_F);
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const int pair = group + i * kSumGroups;
-    const int w2 = pair < kPairs ? *reinterpret_cast<const int*>(w_s + 2 * pair) : 0;
+    const int w2 = *reinterpret_cast<const int*>(w_s + 2 * pair);
     uint32_t a0, a1, b0, b1;
     e2m1x8_twice(v[i][0], a0, a1);
     e2m1x8_twice(v[i][1], b0, b1);
@@ -163,6 +163,117 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
     *reinterpret_cast<uint16_t*>(out + kLatent + 2 * lane) = uint16_t((r[0] & 0xff) | (r[1] & 0xff) << 8);
   }
   if (tid == 0) p.summary_sf[page] = scale;
+}
+
+// Four pages of 8 or 16 tokens a CTA, 64 threads each: a thread has eight dims of all tokens, so that nothing is added up across threads but RoPE, of
+// which it has four dims of every fourth token.
+template <int kPage>
+__global__ void __launch_bounds__(kSumThreads) summarize_four_kernel(SummarizeParams p, int64_t count) {
+  constexpr int kPairs = kPage / 2, kRopeMine = kPage / 4;
+  __shared__ __align__(8) int16_t w_s[4][kPage];
+  __shared__ float top_s[4];
+  __shared__ int rope_s[4][kRope], most_s[4][2], unsound_s[4];
+  __shared__ float scale_s[4], by_s[4][2];
+  dependent_launch();
+  const int tid = threadIdx.x, sub = tid >> 6, t = tid & 63, half = t >> 5, lane = tid & 31;
+  const int64_t item = int64_t(blockIdx.x) * 4 + sub;
+  const int page = item < count ? page_of_item<kPage>(p, item) : -1;
+  const bool there = page >= 0;
+  const uint8_t* rows = p.kv_cache + int64_t(there ? page : 0) * kPage * kRowBytes;
+  const float* scales = p.kv_cache_sf + int64_t(there ? page : 0) * kPage;
+  const float s = there && t < kPage ? __ldcg(scales + t) : 0.f;
+  uint32_t rope[kRopeMine];
+#pragma unroll
+  for (int i = 0; i < kRopeMine; ++i)
+    rope[i] = there ? __ldcg(reinterpret_cast<const uint32_t*>(rows + ((t >> 4) + 4 * i) * kRowBytes + kLatent / 2) + (t & 15)) : 0u;
+  uint32_t v[kPairs][2];
+#pragma unroll
+  for (int i = 0; i < kPage; ++i) v[i >> 1][i & 1] = there ? __ldcg(reinterpret_cast<const uint32_t*>(rows + i * kRowBytes) + t) : 0u;
+  const bool unsound = !(fabsf(s) <= CUDART_MAX_NORMAL_F);
+  // (the page's scales are in its first warp; non-negative floats order as integers)
+  float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(unsound ? 0.f : fabsf(s))));
+  if (t == 0) unsound_s[sub] = 0;
+  if (t == 0) top_s[sub] = top;
+  __syncthreads();
+  top = top_s[sub];
+  if (unsound) unsound_s[sub] = 1;
+  if (t < kPage) w_s[sub][t] = top > 0.f && !unsound ? int16_t(rint(32767.0 * double(s) / double(top))) : int16_t(0);
+  // RoPE: sums of at most four values of at most 448 in steps of 2^-9 are exact in FP32
+  float sum[4] = {};
+#pragma unroll
+  for (int i = 0; i < kRopeMine; ++i) {
+    const float2 a = e4m3x2_to_float2(rope[i] & 0xffff), b = e4m3x2_to_float2(rope[i] >> 16);
+    sum[0] += a.x;
+    sum[1] += a.y;
+    sum[2] += b.x;
+    sum[3] += b.y;
+  }
+  int whole[4];
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    nan |= !(sum[i] == sum[i]);
+    whole[i] = int(512.f * sum[i]);
+    whole[i] += __shfl_xor_sync(0xffffffffu, whole[i], 16);
+  }
+  if (nan) unsound_s[sub] = 1;
+  if (half == 1 && lane < 16) *reinterpret_cast<int4*>(&rope_s[sub][4 * lane]) = make_int4(whole[0], whole[1], whole[2], whole[3]);
+  __syncthreads();
+  int acc[8] = {};
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const int w2 = *reinterpret_cast<const int*>(&w_s[sub][2 * i]);
+    uint32_t a0, a1, b0, b1;
+    e2m1x8_twice(v[i][0], a0, a1);
+    e2m1x8_twice(v[i][1], b0, b1);
+    const uint32_t p01 = __byte_perm(a0, b0, 0x5140), p23 = __byte_perm(a0, b0, 0x7362), p45 = __byte_perm(a1, b1, 0x5140), p67 = __byte_perm(a1, b1, 0x7362);
+    acc[0] = dp2a_lo(w2, p01, acc[0]);
+    acc[1] = dp2a_hi(w2, p01, acc[1]);
+    acc[2] = dp2a_lo(w2, p23, acc[2]);
+    acc[3] = dp2a_hi(w2, p23, acc[3]);
+    acc[4] = dp2a_lo(w2, p45, acc[4]);
+    acc[5] = dp2a_hi(w2, p45, acc[5]);
+    acc[6] = dp2a_lo(w2, p67, acc[6]);
+    acc[7] = dp2a_hi(w2, p67, acc[7]);
+  }
+  int most = 0, most_rope = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, abs(acc[i]));
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (half == 0) {  // (lanes 0-15 and 16-31 have the same sums)
+    const int4 more = *reinterpret_cast<const int4*>(&rope_s[sub][4 * (lane & 15)]);
+    whole[0] += more.x;
+    whole[1] += more.y;
+    whole[2] += more.z;
+    whole[3] += more.w;
+    most_rope = __reduce_max_sync(0xffffffffu, max(max(abs(whole[0]), abs(whole[1])), max(abs(whole[2]), abs(whole[3]))));
+  }
+  if (lane == 0) most_s[sub][half] = most;
+  __syncthreads();
+  constexpr double kLatUnit = 1.0 / (65534.0 * kPage), kRopeUnit = 1.0 / (512.0 * kPage);
+  if (half == 0) {
+    const float scale = unsound_s[sub] ? CUDART_NAN_F : summary_scale(max(most_s[sub][0], most_s[sub][1]), most_rope, top, kLatUnit, kRopeUnit);
+    if (lane == 0) {
+      scale_s[sub] = scale;
+      by_s[sub][0] = top / scale * float(kLatUnit);
+      by_s[sub][1] = float(kRopeUnit) / scale;
+      if (there) p.summary_sf[page] = scale;
+    }
+  }
+  __syncthreads();
+  if (!there) return;
+  const float scale = scale_s[sub], by = by_s[sub][0];
+  int8_t* out = p.summary + int64_t(page) * kQDim;
+  uint32_t code[2] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) code[i >> 2] |= uint32_t(summary_code(acc[i], scale, by, top, kLatUnit) & 0xff) << (8 * (i & 3));
+  *reinterpret_cast<uint2*>(out + 8 * t) = make_uint2(code[0], code[1]);
+  if (half == 0 && lane < 16) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= uint32_t(summary_code(whole[i], scale, by_s[sub][1], 1.f, kRopeUnit) & 0xff) << (8 * i);
+    *reinterpret_cast<uint32_t*>(out + kLatent + 4 * lane) = r;
+  }
 }
 
 // ------------------------------------------------------------------------------------------ selection
@@ -317,16 +428,22 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
 
 }  // namespace
 
-// From how many tokens on pages go to summarize_many_kernel, this kernel -> that one, us: pages of 64 tokens, 76000 tokens 11.1 -> 11.8, 150000
-// 18.3 -> 16.6, 300000 32.6 -> 26.3; of 32, 12.4 -> 13.9, 21.3 -> 19.5, 39.6 -> 32.5; of 128, 11.0 -> 11.2, 17.0 -> 15.6, 28.2 -> 24.2.  Pages of 16
-// tokens, eight to a tile, took longer there whatever their number (300000 tokens 64.3 -> 73.4), and so did those of 8 (116.4 -> 120.3).
-constexpr int64_t kManyTokens = 131072;
-constexpr int kManyPage = 32;
+// Which kernel, us in graphs of calls on pages that are not in L2, for 4096 / 38000 / 150000 / 300000 tokens (a CTA per page, four pages a CTA, many):
+//   pages of   8   3.6 / 16.8 / 59.5 / 116     3.4 /  9.0 / 26.5 / 50.1    (sixteen pages to a tile) 12 / 25 / 65 / 120
+//             16   3.7 / 10.4 / 33.5 / 64.3    3.2 /  7.9 / 21.2 / 38.3    (eight) 8.3 / 16.2 / 38.8 / 73.4
+//             32   3.0 /  7.4 / 21.3 / 39.6    3.9 /  9.7 / 18.7 / 33.0    6.4 / 10.0 / 19.5 / 32.5
+//             64   3.1 /  6.6 / 18.3 / 32.6    5.3 /  9.7 / 17.2 / 29.0    5.2 /  8.3 / 16.6 / 26.3
+//            128   3.5 /  6.4 / 17.0 / 28.2    8.4 / 11.2 / 22.6 / 30.3    4.9 /  7.3 / 15.6 / 24.2
+// With small pages what is done once a page outweighs its sums, and four share it; with large ones four in turn are longer than one by four groups.
+constexpr int64_t kManyTokens = 131072;  // (76000: 11.1 with a CTA per page, 11.8)
 
 cudaError_t launch_summarize(const SummarizeParams& p, int64_t count, int sms, cudaStream_t stream) {
-  if (p.page_size >= kManyPage && count * p.page_size >= kManyTokens && reinterpret_cast<uintptr_t>(p.kv_cache) % 32 == 0) return launch_summarize_many(p, count, sms, stream);
-  const auto kernel = p.page_size == 8 ? summarize_kernel<8> : p.page_size == 16 ? summarize_kernel<16> : p.page_size == 32 ? summarize_kernel<32>
-                      : p.page_size == 64 ? summarize_kernel<64> : summarize_kernel<128>;
+  if (p.page_size <= 16) {
+    const auto kernel = p.page_size == 8 ? summarize_four_kernel<8> : summarize_four_kernel<16>;
+    return launch_dependent(kernel, dim3(unsigned((count + 3) / 4)), kSumThreads, 0, stream, p, count);
+  }
+  if (count * p.page_size >= kManyTokens && reinterpret_cast<uintptr_t>(p.kv_cache) % 32 == 0) return launch_summarize_many(p, count, sms, stream);
+  const auto kernel = p.page_size == 32 ? summarize_kernel<32> : p.page_size == 64 ? summarize_kernel<64> : summarize_kernel<128>;
   return launch_dependent(kernel, dim3(unsigned(count)), kSumThreads, 0, stream, p);
 }
 
