@@ -3,8 +3,10 @@
 // Pages are the M axis: a thread of the epilogue has a page (a TMEM lane) and goes over its heads in registers; with the heads on M the
 // largest over heads would be a reduction across threads, and fewer than 128 heads would waste half of the MMA or more.
 //
-// Bound by HBM: a page's 580 bytes are read once per query position, an SM's share of the measured copy rate is a tile (128 pages, 74 KB) in
-// 1.7 us, and its 18 MMAs of 128 x 128 x 32 take less.  So a CTA per SM walks a contiguous range of the tiles of all rows, in two stages of a
+// Bound by the gather of the pages' rows: 580 bytes a page and query position, an SM's share of the measured copy rate is a tile (128 pages,
+// 74 KB) in 1.7 us, and its 18 MMAs of 128 x 128 x 32 take 0.9.  64 requests of 2048 pages, 128 heads: 24 us behind other kernels, of
+// which 6 are the first two tiles and the queries (4.3 TB/s from all SMs at once), 1.7 their conversion, then 2.6 a tile (4.2 TB/s); a
+// kernel that does nothing but read the same rows by number takes 22.3.  So a CTA per SM walks a contiguous range of the tiles of all rows, in two stages of a
 // whole tile each: at least one tile is in flight whatever the other roles do.  Rows come by cp.async straight into the
 // 64-byte swizzle of the operand (576 = 9 x 64 without a rest; eight rows x 64 bytes per instruction are one swizzle atom: no bank
 // conflicts, whole sectors); a TMA gather would take 288 instructions of 256 bytes a tile.
@@ -369,7 +371,8 @@ static_assert(1024 + kStages * kStageBytes + 128 * kQDim + sizeof(Small) <= 2324
 cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream) {
   const int rows = p.batch * p.q_len, columns = (p.heads + 15) / 16 * 16;
   const size_t smem = smem_bytes(columns);
-  cudaError_t e = cudaFuncSetAttribute(score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_bytes(128)));
+  static std::atomic<bool> allowed[64];
+  cudaError_t e = allow_smem(score_kernel, smem_bytes(128), allowed);
   if (e != cudaSuccess) return e;
   const int64_t tiles = (p.width - p.sink - p.local + kPages - 1) / kPages;  // of the longest row that the tables can hold
   for (int row0 = 0; row0 < rows; row0 += kMaxRows) {

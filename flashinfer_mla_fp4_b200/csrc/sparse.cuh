@@ -3,6 +3,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "launch.h"
 
@@ -37,6 +39,19 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two_bytes) {
   const uint32_t h = e4m3x2_to_f16x2(two_bytes);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// Allows a kernel that much dynamic shared memory, once per device (setting it twice is harmless).
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, size_t bytes, std::atomic<bool> (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess && known) done[dev].store(true, std::memory_order_release);
+  return e;
 }
 
 // What a query position sees of its request.

@@ -319,7 +319,8 @@ cudaError_t launch(const SummarizeParams& p, int64_t count, int sms, cudaStream_
   CUtensorMap latent, rope;
   if (!encode_latent_map(p.kv_cache, p.num_pages, kPage, kPage, &latent) || !encode_rope_map(p.kv_cache, p.num_pages, kPage, kPage, false, &rope))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(summarize_many_kernel<kPage>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes));
+  static std::atomic<bool> allowed[64];
+  cudaError_t e = allow_smem(summarize_many_kernel<kPage>, kSmemBytes, allowed);
   if (e != cudaSuccess) return e;
   const int64_t tiles = (count + kTile / kPage - 1) / (kTile / kPage);
   return launch_dependent(summarize_many_kernel<kPage>, dim3(unsigned(tiles < sms ? tiles : sms)), kThreads, kSmemBytes, stream, p, count, latent, rope);

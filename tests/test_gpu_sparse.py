@@ -493,3 +493,107 @@ def test_a_backend_with_sparse_pages_over_growing_requests(graph):
             ref, _ = _expected(cache, bt, sl, q, ps, budget, 1, 2, False, scale)
             O.assert_parity(out.float().cpu(), ref, f"step {i}")
     assert pool.num_free() == 140 - len({p for b, n in enumerate(sl.tolist()) for p in bt[b, : -(-n // ps)].tolist()})
+
+
+def test_page_ids_are_validated_on_demand(monkeypatch):
+    cache, bt, sl, q = _sparse_case([900, 700], 16, 16, 1, seed=6)
+    w = _wrapper(num_heads=16, page_size=16, budget_pages=8)
+    args = (q, cache.kv_cache, bt, sl, 900, 0.05)
+    kw = dict(kv_cache_sf=cache.kv_cache_sf, summary=cache.summary, summary_sf=cache.summary_sf)
+    want = w.run(*args, **kw)
+    monkeypatch.setenv("MLA_FP4_VALIDATE", "1")
+    assert torch.equal(w.run(*args, **kw), want)
+    bt[1, 20] = cache.num_pages
+    with pytest.raises(ValueError, match=r"block_tables\[1, 20\]"):
+        w.run(*args, **kw)
+
+
+def test_offsets_beyond_32_bits():
+    """Pages at the far end of caches and summaries of more than 2^31 bytes."""
+    dev = _dev()
+    from flashinfer_mla_fp4_b200.sparse import select_pages, summarize_pages
+
+    pool, page, some = 3_900_000, 8, 300  # summaries of 2.2 GB
+    far = 900_000  # pages of the cache: 2.3 GB
+    kv, sf = _pages(some, page, 77)
+    cache, scales = torch.zeros(far, page, 320, dtype=torch.uint8, device=dev), torch.zeros(far, page, 1, device=dev)
+    cache[-some:], scales[-some:] = kv.to(dev), sf.to(dev)
+    summary, ssf = torch.zeros(far, 576, dtype=torch.int8, device=dev), torch.zeros(far, device=dev)
+    summarize_pages(cache, scales, summary, ssf, torch.arange(far - some, far, dtype=torch.int32, device=dev))
+    codes, want_sf = _oracle_summaries(kv, sf)
+    assert torch.equal(summary[-some:].cpu(), codes) and torch.equal(ssf[-some:].cpu(), want_sf)
+    assert not bool(summary[:-some].any())
+    big, big_sf = torch.zeros(pool, 576, dtype=torch.int8, device=dev), torch.zeros(pool, device=dev)
+    big[-some:], big_sf[-some:] = summary[-some:], ssf[-some:]
+    q = torch.randn(1, 1, 24, 576, generator=torch.Generator().manual_seed(1)).to(E4M3)
+    order = torch.randperm(some, generator=torch.Generator().manual_seed(2)).int().view(1, -1)
+    sl = torch.tensor([some * page], dtype=torch.int32)
+    want, _ = S.select(q, codes, want_sf, order, sl, page, 30, 1, 2, False)
+    got, _ = select_pages(q.to(dev), big, big_sf, (order + (pool - some)).int().to(dev), sl.to(dev), page, 30)
+    assert torch.equal(got.cpu(), want + (pool - some))
+
+
+def test_empty_batches_and_tables():
+    dev = _dev()
+    from flashinfer_mla_fp4_b200.sparse import select_pages, summarize_new_pages
+
+    cache, bt, sl, q = _sparse_case([900], 16, 16, 1, seed=6)
+    sel, lens = select_pages(q[:0], cache.summary, cache.summary_sf, bt[:0], sl[:0], 16, 8)
+    assert sel.shape == (0, 8) and lens.shape == (0,)
+    sel, lens = select_pages(q, cache.summary, cache.summary_sf, bt[:, :0], sl, 16, 8)
+    assert sel.tolist() == [[0] * 8] and lens.tolist() == [0]
+    summarize_new_pages(cache.kv_cache, cache.kv_cache_sf, cache.summary, cache.summary_sf, bt[:, :0], sl, 5)
+    summarize_new_pages(cache.kv_cache, cache.kv_cache_sf, cache.summary, cache.summary_sf, bt, sl, 0)
+    torch.cuda.synchronize()
+
+
+_FIRST = """
+import sys, torch
+sys.path.insert(0, {root!r})
+sys.path.insert(0, {tests!r})
+import test_gpu_sparse as T
+from flashinfer_mla_fp4_b200 import FP4MLAPagedCache, FP4MLAPagePool
+from flashinfer_mla_fp4_b200.sparse import select_pages, summarize_pages
+dev = torch.device("cuda:0")
+q, summary, ssf, bt, sl = (t.to(dev) for t in T._selection_case([3000, 2000], 24, 16, 1, seed=9))
+kv, sf = T._pages(8200, 16, 3)
+kv, sf = kv.to(dev), sf.to(dev)
+kv64, sf64 = kv.view(-1, 64, 320), sf.view(-1, 64, 1)
+out = [torch.zeros(n, 576, dtype=torch.int8, device=dev) for n in (8200, 2050, 2050)]
+out_sf = [torch.zeros(n, device=dev) for n in (8200, 2050, 2050)]
+ids, ids64 = torch.arange(8200, dtype=torch.int32, device=dev), torch.arange(2050, dtype=torch.int32, device=dev)
+pool = FP4MLAPagePool([FP4MLAPagedCache(40, 16, dev)])
+table, lens, ask = torch.zeros(2, 4, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev), torch.tensor([40, 0], dtype=torch.int32, device=dev)
+zero, one = torch.zeros(1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = select_pages(q, summary, ssf, bt, sl, 16, 20)
+    summarize_pages(kv, sf, out[0], out_sf[0], ids)
+    summarize_pages(kv64, sf64, out[1], out_sf[1], ids64)
+    summarize_pages(kv64, sf64, out[2], out_sf[2], ids64[:64])
+    pool.allocate(table, lens, ask)
+    lens.copy_(ask)
+    pool.fork(table, lens, zero, one)
+    pool.free(table, lens, zero)
+    pool.compact(table, lens)
+graph.replay()
+torch.cuda.synchronize()
+again = select_pages(q, summary, ssf, bt, sl, 16, 20)
+assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+assert torch.equal(out[1][:64], out[2][:64]) and bool(out[0].any())
+assert lens.tolist() == [0, 40] and pool.refcounts.tolist()[:3] == [1, 1, 1] and pool.num_free() == 37
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    """No kernel has run before its first call is recorded."""
+    _dev()
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    here = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", _FIRST.format(root=str(here.parent), tests=str(here))], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
