@@ -598,7 +598,8 @@ int pool_params(const MlaFp4PoolArgs* a, int32_t count, mla::PoolParams* p) {
     snprintf(buf, sizeof buf, "workspace has %zu bytes, but %zu are required", a->workspace ? a->workspace_bytes : size_t(0), need);
     return fail(MLA_FP4_ERR_WORKSPACE_TOO_SMALL, buf);
   }
-  if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(MLA_FP4_ERR_BAD_ARG, "workspace must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 16 || reinterpret_cast<uintptr_t>(a->refcounts) % 16)
+    return fail(MLA_FP4_ERR_BAD_ARG, "workspace and refcounts must be 16-byte aligned");
   p->refcounts = a->refcounts; p->block_tables = a->block_tables; p->seq_lens = a->seq_lens;
   p->ws = static_cast<int32_t*>(a->workspace); p->status = a->status;
   p->num_pages = a->num_pages; p->block_table_stride = a->block_table_stride;

@@ -137,7 +137,8 @@ struct SelectParams {
   uint32_t wait_polls;
   int32_t* status;
 };
-cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream);   // score_sm100.cu: the keys
+cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream);   // score_sm100.cu: the keys, or, if so, the selection
+bool scores_and_selects(const SelectParams& p, int sms);
 cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream);  // keys and selection
 // pages.cu
 struct PageLayer {  // the caches of a layer; summary may be null

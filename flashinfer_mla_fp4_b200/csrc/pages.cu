@@ -51,24 +51,38 @@ __device__ __forceinline__ T scan_before(T v, T* warp_s, T* total) {
   return sum - v + (warp ? warp_s[warp - 1] : 0);
 }
 
+constexpr int kPerThread = 8;  // counts that a thread of a planning CTA looks at in a round: two loads of 16 bytes
+constexpr int kPerRound = kPlanThreads * kPerThread;
+
+// Reference counts first + 8 tid to + 7 (1, in use, behind the last one).
+struct Counts {
+  int32_t n[kPerThread];
+  __device__ __forceinline__ Counts(const int32_t* refcounts, int64_t first, int64_t num_pages) {
+    const int64_t at = first + threadIdx.x * kPerThread;
+    if (at + kPerThread <= num_pages) {
+#pragma unroll
+      for (int i = 0; i < kPerThread; i += 4) *reinterpret_cast<int4*>(n + i) = __ldcg(reinterpret_cast<const int4*>(refcounts + at + i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) n[i] = at + i < num_pages ? __ldcg(refcounts + at + i) : 1;
+    }
+  }
+};
+
 // Calls take(number, page) for the free pages of the lowest numbers, the first `wanted` of them; returns how many there were.
 template <typename Take>
 __device__ __forceinline__ int for_free_pages(const int32_t* refcounts, int64_t num_pages, int wanted, int* warp_s, Take take) {
   int found = 0;
-  for (int64_t base = 0; base < num_pages && found < wanted; base += kPlanThreads * 4) {
-    const int64_t at = base + threadIdx.x * 4;
-    bool free[4];
+  for (int64_t base = 0; base < num_pages && found < wanted; base += kPerRound) {
+    const Counts c(refcounts, base, num_pages);
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      free[i] = at + i < num_pages && refcounts[at + i] <= 0;
-      n += free[i];
-    }
+    for (int i = 0; i < kPerThread; ++i) n += c.n[i] <= 0;
     int total, number = found + scan_before(n, warp_s, &total);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (free[i]) {
-        if (number < wanted) take(number, int(at + i));
+    for (int i = 0; i < kPerThread; ++i)
+      if (c.n[i] <= 0) {
+        if (number < wanted) take(number, int(base) + int(threadIdx.x) * kPerThread + i);
         ++number;
       }
     found += total;
@@ -251,18 +265,33 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PoolParams p
   dependent_launch();
   int32_t *hole = p.ws + 4, *high = hole + p.num_pages;
   int mine = 0, live;
-  for (int64_t i = threadIdx.x; i < p.num_pages; i += kPlanThreads) mine += p.refcounts[i] > 0;
+  for (int64_t base = 0; base < p.num_pages; base += kPerRound) {
+    const Counts c(p.refcounts, base, p.num_pages);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) mine += c.n[i] > 0 && base + threadIdx.x * kPerThread + i < p.num_pages;
+  }
   scan_before(mine, warp_s, &live);
   int holes = 0, highs = 0;
-  for (int64_t base = 0; base < p.num_pages; base += kPlanThreads) {
-    const int64_t i = base + threadIdx.x;
-    const bool in = i < p.num_pages, used = in && p.refcounts[i] > 0;
-    const int a = in && !used && i < live, b = used && i >= live;
+  for (int64_t base = 0; base < p.num_pages; base += kPerRound) {
+    const Counts c(p.refcounts, base, p.num_pages);
+    const int64_t at = base + threadIdx.x * kPerThread;
+    int both = 0;  // holes, and pages that move in the upper half
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const bool used = c.n[i] > 0, low = at + i < live;
+      both += (!used && low ? 1 : 0) + (used && !low && at + i < p.num_pages ? 1 << 16 : 0);
+    }
     int sum;
-    const int before = scan_before(a | (b << 16), warp_s, &sum);
-    if (a) hole[holes + (before & 0xffff)] = int(i);
-    if (b) high[highs + (before >> 16)] = int(i);
-    if (in) remap[i] = used ? int(i) : -1;
+    const int before = scan_before(both, warp_s, &sum);
+    int h = holes + (before & 0xffff), m = highs + (before >> 16);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      if (at + i >= p.num_pages) break;
+      const bool used = c.n[i] > 0, low = at + i < live;
+      if (!used && low) hole[h++] = int(at) + i;
+      if (used && !low) high[m++] = int(at) + i;
+      remap[at + i] = used ? int(at) + i : -1;
+    }
     holes += sum & 0xffff;
     highs += sum >> 16;
   }

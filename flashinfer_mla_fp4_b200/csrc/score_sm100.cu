@@ -11,6 +11,9 @@
 // 64-byte swizzle of the operand (576 = 9 x 64 without a rest; eight rows x 64 bytes per instruction are one swizzle atom: no bank
 // conflicts, whole sectors); a TMA gather would take 288 instructions of 256 bytes a tile.
 //
+// Few rows of one tile each (score_kernel<true>): a CTA has a row to itself, keeps its keys in shared memory and selects too, by counting for each page
+// those before it: no second launch, and nothing that another CTA has to see.
+//
 // Roles: warps 0-3 take the scores out of TMEM, warp 4 issues the MMAs, warps 5-12 load, and turn a row's query into integers (the B
 // operand) while the row's first two tiles are on their way.  All waits are bounded; one that runs out sets the status and ends the CTA, whose
 // keys are then not all written.
@@ -33,10 +36,13 @@ constexpr int kStageBytes = kPages * kQDim;       // [9 blocks][128 pages][64 by
 constexpr int kStages = 2;
 constexpr int kMaxRows = 1024;                    // rows of a launch (the launcher makes several)
 constexpr uint32_t kTmemCols = 256;               // two accumulators of up to 128 columns
+constexpr int kWholeKeys = kPages;                // most candidates of a row that a CTA has to itself
 
 // shared memory, from a 1024-byte boundary on: the stages, the query's codes [9][columns][64 bytes], then
 struct Small {
   int candidates[kMaxRows];  // pages that a row scores
+  alignas(16) uint32_t keys[kWholeKeys];  // of a row that the CTA has to itself
+  int taken[kWholeKeys / 32];
   float unit[4][128];        // 2^-k of the heads, by row: an epilogue may be three tiles, so three rows, behind the loads
   unsigned long long full_a[kStages], empty_a[kStages], full_d[2], empty_d[2], full_b, drained;
   uint32_t tmem;
@@ -177,6 +183,45 @@ __device__ __forceinline__ void convert_b(char* b_smem, float* unit, int columns
   }
 }
 
+// The selection of a row by the CTA that has its keys in shared memory.  The place of a page is the number of those with a larger key, or with the
+// same one and nearer the start: 128 compares per thread, with four keys a load that all threads share.
+__device__ __forceinline__ void select_whole(const SelectParams& p, Small& s, int row, const Seen& v, int page) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int32_t* table = p.block_tables + int64_t(row / p.q_len) * p.block_table_stride;
+  int32_t* out = p.selected + int64_t(row) * p.budget;
+  if (v.used <= p.budget) {  // the budget holds them all
+    for (int k = tid; k < p.budget; k += kThreads) out[k] = k < v.used ? __ldcg(table + k) : 0;
+    if (tid == 0) p.selected_lens[row] = v.len;
+    return;
+  }
+  const int candidates = v.used - p.sink - p.local, wanted = p.budget - p.sink - p.local;
+  for (int k = tid; k < p.sink; k += kThreads) out[k] = __ldcg(table + k);
+  for (int k = tid; k < p.local; k += kThreads) out[p.budget - p.local + k] = __ldcg(table + v.used - p.local + k);
+  if (tid == 0) p.selected_lens[row] = v.len - (v.used - p.budget) * p.page_size;
+  bool take = false;
+  uint32_t ballot = 0;
+  if (warp < kWholeKeys / 32) {
+    const uint32_t key = s.keys[tid];
+    int before = 0;
+#pragma unroll 4
+    for (int k = 0; k < candidates; k += 4) {  // (behind the candidates the keys are 0, and their places behind every candidate's)
+      const uint4 four = *reinterpret_cast<const uint4*>(s.keys + k);
+      before += (four.x > key || (four.x == key && k < tid)) + (four.y > key || (four.y == key && k + 1 < tid)) +
+                (four.z > key || (four.z == key && k + 2 < tid)) + (four.w > key || (four.w == key && k + 3 < tid));
+    }
+    take = tid < candidates && before < wanted;
+    ballot = __ballot_sync(0xffffffffu, take);
+    if (lane == 0) s.taken[warp] = __popc(ballot);
+  }
+  __syncthreads();
+  if (!take) return;
+  int at = p.sink + __popc(ballot & ((1u << lane) - 1));
+  for (int w = 0; w < warp; ++w) at += s.taken[w];
+  out[at] = page;
+}
+
+// kWhole: CTA i has row i and selects; else the CTAs share the tiles of rows row0 to row0 + rows - 1.
+template <bool kWhole>
 __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int row0, int rows, int columns) {
   extern __shared__ char raw[];
   char* a_smem = raw + ((1024 - (ptx::smem_u32(raw) & 1023)) & 1023);
@@ -204,15 +249,32 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int r = tid; r < rows; r += kThreads) {
-    const Seen v = seen(p, row0 + r);
-    s.candidates[r] = v.used > p.budget ? v.used - p.sink - p.local : 0;
+  Seen mine{0, 0};
+  int page_of_mine = 0;  // of the candidate that this thread may take
+  if constexpr (kWhole) {
+    row0 = blockIdx.x;
+    mine = seen(p, row0);
+    const int candidates = mine.used > p.budget ? mine.used - p.sink - p.local : 0;
+    if (tid == 0) {
+      s.candidates[0] = candidates;
+      s.first_row = s.first_tile = 0;
+      s.tiles = (candidates + kPages - 1) / kPages;
+    }
+    if (tid < kWholeKeys) {
+      s.keys[tid] = 0;
+      if (tid < candidates) page_of_mine = __ldcg(p.block_tables + int64_t(row0 / p.q_len) * p.block_table_stride + p.sink + tid);
+    }
+  } else {
+    for (int r = tid; r < rows; r += kThreads) {
+      const Seen v = seen(p, row0 + r);
+      s.candidates[r] = v.used > p.budget ? v.used - p.sink - p.local : 0;
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = s.tmem;
-  if (warp == 0) {  // this CTA's share: tiles [T i / n, T (i + 1) / n) of all tiles in the order of the rows
+  if (!kWhole && warp == 0) {  // this CTA's share: tiles [T i / n, T (i + 1) / n) of all tiles in the order of the rows
     long long total = 0;
     for (int base = 0; base < rows; base += 32)
       total += __reduce_add_sync(0xffffffffu, base + lane < rows ? (s.candidates[base + lane] + kPages - 1) / kPages : 0);
@@ -251,21 +313,23 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       bool ok = true;
       for (int n = 0; ; ++n) {
         const int st = n & 1;
-        if (n >= kStages) ok = wait(c, s.empty_a[st], ((n >> 1) - 1) & 1);
+        const bool more = k.left > 0;
+        if (n >= kStages && (more || fresh >= 0)) ok = wait(c, s.empty_a[st], ((n >> 1) - 1) & 1);
         if (!ok) break;
         if (fresh >= 0 && seg > 0) {
           fetch_b(p, b_addr, row0 + fresh, columns);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        const bool more = k.left > 0;
         const int next_fresh = more && (n == 0 || k.tile == 0) ? k.row : -1;
         if (more) {
           k.next();
-          const int page = next_page >= 0 && next_page < p.num_pages ? next_page : 0;  // (0 for one that nobody reads)
+          const int page = next_page < p.num_pages ? next_page : -1;
           next_page = lane < kMine ? k.entry(p, row0, first + lane) : -1;
+          // (rows without a page are left as they are: what comes of them nobody reads.  With some page in their place, the same for all, the tiles
+          // that are not full had all SMs wait for one line: 148 rows of 57 candidates 21.2 us instead of 11.5.)
           for_chunks(kMine, [&](int r, int chunk) {
             const int from = __shfl_sync(0xffffffffu, page, r);
-            cp_async16(a_addr + st * kStageBytes + operand_at(kPages, first + r, chunk), p.summary + int64_t(from) * kQDim + 16 * chunk);
+            if (from >= 0) cp_async16(a_addr + st * kStageBytes + operand_at(kPages, first + r, chunk), p.summary + int64_t(from) * kQDim + 16 * chunk);
           });
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -328,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       int seg = 0, next_page = k.entry(p, row0, tid);
       for (int n = 0; k.left > 0; ++n) {
         const int st = n & 1, row = k.row, i = k.tile * kPages + tid, page = next_page;
-        const bool mine = i < k.candidates[row], last = k.row_ends(), there = page >= 0 && page < p.num_pages;
+        const bool scored = i < k.candidates[row], last = k.row_ends(), there = page >= 0 && page < p.num_pages;
         const float scale = there ? __ldcg(p.summary_sf + page) : 0.f;
         k.next();
         next_page = k.entry(p, row0, tid);
@@ -350,7 +414,9 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(s.empty_d[st]));
-        if (mine) p.keys[int64_t(row0 + row) * p.key_stride + i] = there ? key_of(best * scale) : 0u;
+        const uint32_t key = there ? key_of(best * scale) : 0u;
+        if (kWhole && scored) s.keys[i] = key;
+        if (!kWhole && scored) p.keys[int64_t(row0 + row) * p.key_stride + i] = key;
         seg += last;
       }
     }
@@ -361,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, kTmemCols);
   }
+  if constexpr (kWhole) select_whole(p, s, row0, mine, page_of_mine);
 }
 
 size_t smem_bytes(int columns) { return 1024 + size_t(kStages) * kStageBytes + size_t(columns) * kQDim + sizeof(Small); }
@@ -368,17 +435,24 @@ static_assert(1024 + kStages * kStageBytes + 128 * kQDim + sizeof(Small) <= 2324
 
 }  // namespace
 
+// Rows with at most 128 candidates have a CTA each that selects too, us in graphs, a launch each for scores and selection -> this: 16 heads, 57
+// candidates, 1 row 9.3 -> 6.9, 148 rows 11.5 -> 7.8, 296 15.9 -> 15.1; 128 heads, 127 candidates, 11.7 -> 10.1, 14.2 -> 11.0, 21.2 -> 21.6: so while
+// there are no more rows than SMs.  With two tiles, and the compares of 256 keys with one another, it was 9.6 -> 10.9.
+bool scores_and_selects(const SelectParams& p, int sms) { return p.width - p.sink - p.local <= kWholeKeys && p.batch * p.q_len <= sms; }
+
 cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream) {
   const int rows = p.batch * p.q_len, columns = (p.heads + 15) / 16 * 16;
   const size_t smem = smem_bytes(columns);
-  static std::atomic<bool> allowed[64];
-  cudaError_t e = allow_smem(score_kernel, smem_bytes(128), allowed);
+  static std::atomic<bool> allowed[2][64];
+  cudaError_t e = allow_smem(score_kernel<false>, smem_bytes(128), allowed[0]);
+  if (e == cudaSuccess) e = allow_smem(score_kernel<true>, smem_bytes(128), allowed[1]);
   if (e != cudaSuccess) return e;
+  if (scores_and_selects(p, sms)) return launch_dependent(score_kernel<true>, dim3(unsigned(rows)), kThreads, smem, stream, p, 0, 1, columns);
   const int64_t tiles = (p.width - p.sink - p.local + kPages - 1) / kPages;  // of the longest row that the tables can hold
   for (int row0 = 0; row0 < rows; row0 += kMaxRows) {
     const int n = rows - row0 < kMaxRows ? rows - row0 : kMaxRows;
     const int64_t most = tiles * n;
-    e = launch_dependent(score_kernel, dim3(unsigned(most < sms ? most : sms)), kThreads, smem, stream, p, row0, n, columns);
+    e = launch_dependent(score_kernel<false>, dim3(unsigned(most < sms ? most : sms)), kThreads, smem, stream, p, row0, n, columns);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

@@ -450,7 +450,7 @@ cudaError_t launch_summarize(const SummarizeParams& p, int64_t count, int sms, c
 cudaError_t launch_select(const SelectParams& p, int sms, cudaStream_t stream) {
   if (p.width > p.budget) {
     cudaError_t e = launch_score(p, sms, stream);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || scores_and_selects(p, sms)) return e;
   }
   // keys of the longest row that the tables can hold: four a thread while there are threads, then sixteen (none where the budget holds every row)
   const int rows = p.batch * p.q_len, most = p.width - p.sink - p.local;

@@ -355,12 +355,12 @@ typedef struct MlaFp4PoolArgs {
   const MlaFp4PageLayer* layers; /* on the host */
   int32_t num_layers, page_size;
   int64_t num_pages;
-  int32_t* refcounts;
+  int32_t* refcounts;            /* 16-byte aligned */
   int32_t* block_tables;
   int64_t block_table_stride;
   int32_t width, rows;
   int32_t* seq_lens;
-  void* workspace; /* mla_fp4_pool_workspace_bytes; 4-byte aligned; nothing is kept in it */
+  void* workspace; /* mla_fp4_pool_workspace_bytes; 16-byte aligned; nothing is kept in it */
   size_t workspace_bytes;
   int32_t* status;
   void* stream;

@@ -115,7 +115,7 @@ def test_more_layers_than_a_launch_takes():
     _check(pool, caches, before, want, bt, sl)
 
 
-@pytest.mark.parametrize("seed,page,layers,pages,rows,width", [(1, 8, 1, 30, 5, 8), (2, 16, 2, 5000, 40, 200), (3, 64, 1, 300, 1100, 3),
+@pytest.mark.parametrize("seed,page,layers,pages,rows,width", [(1, 8, 1, 30, 5, 8), (6, 8, 1, 20001, 50, 900), (7, 8, 1, 8192, 20, 700), (2, 16, 2, 5000, 40, 200), (3, 64, 1, 300, 1100, 3),
                                                               (4, 128, 3, 64, 9, 12), (5, 32, 1, 9000, 2100, 6)])
 def test_random_histories(seed, page, layers, pages, rows, width):
     """Allocations, forks, frees and compactions in any order, with lists that repeat rows, name none, and ask for too much."""
