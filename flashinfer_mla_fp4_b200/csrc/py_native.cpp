@@ -611,20 +611,20 @@ PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// pool(what, layers, num_layers, page_size, refcounts, status, block_tables, seq_lens, x, y): what is 0 allocate (x: new_lens), 1 fork (parents,
+// pool(what, layers, num_layers, page_size, num_pages, refcounts, status, block_tables, seq_lens, x, y): what is 0 allocate (x: new_lens), 1 fork (parents,
 // children), 2 free (x: rows), 3 compact (x: remap or None); layers is the address of the host array -> remap of a compaction, else True; None
 // when the call is not of the common form
 PyObject* pool(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 10) return PyErr_Format(PyExc_TypeError, "pool takes 10 arguments");
-  int64_t what, layers, page;
-  const at::Tensor *ref = tensor(a[4]), *status = tensor(a[5]), *bt = tensor(a[6]), *sl = tensor(a[7]), *x = tensor(a[8]), *y = tensor(a[9]);
-  if (!integer(a[0], &what) || !integer(a[2], &layers) || !integer(a[3], &page) || !ref || !status || !bt || !sl) Py_RETURN_NONE;
+  if (n != 11) return PyErr_Format(PyExc_TypeError, "pool takes 11 arguments");
+  int64_t what, layers, page, pages;
+  const at::Tensor *ref = tensor(a[5]), *status = tensor(a[6]), *bt = tensor(a[7]), *sl = tensor(a[8]), *x = tensor(a[9]), *y = tensor(a[10]);
+  if (!integer(a[0], &what) || !integer(a[2], &layers) || !integer(a[3], &page) || !integer(a[4], &pages) || !ref || !status || !bt || !sl) Py_RETURN_NONE;
   const void* array = PyLong_AsVoidPtr(a[1]);
   if (!array) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "null address");
   const at::Device dev = status->device();
-  const int64_t pages = ref->numel(), rows = bt->size(0);
-  if (!plain(*ref, at::kInt, {-1}, dev) || !tables_ok(*bt, *sl, dev) || rows == 0 || rows > INT32_MAX || (rows > 1 && bt->stride(0) < bt->size(1))) Py_RETURN_NONE;
+  const int64_t rows = bt->size(0);
+  if (!plain(*ref, at::kInt, {pages}, dev) || !tables_ok(*bt, *sl, dev) || rows == 0 || rows > INT32_MAX || (rows > 1 && bt->stride(0) < bt->size(1))) Py_RETURN_NONE;
   int64_t count = 0;
   if (what == 0) {
     if (!x || !plain(*x, at::kInt, {rows}, dev)) Py_RETURN_NONE;
@@ -632,7 +632,7 @@ PyObject* pool(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!x || !plain(*x, at::kInt, {-1}, dev) || x->numel() == 0 || x->numel() > INT32_MAX) Py_RETURN_NONE;
     count = x->numel();
     if (what == 1 && (!y || !plain(*y, at::kInt, {count}, dev))) Py_RETURN_NONE;
-  } else if (a[8] != Py_None && (!x || !plain(*x, at::kInt, {pages}, dev))) {
+  } else if (a[9] != Py_None && (!x || !plain(*x, at::kInt, {pages}, dev))) {
     Py_RETURN_NONE;
   }
   size_t need = 0;
@@ -667,7 +667,7 @@ PyObject* pool(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   if (rc != MLA_FP4_OK) return raise_status(rc);
   if (what != 3) Py_RETURN_TRUE;
-  return x ? Py_NewRef(a[8]) : THPVariable_Wrap(std::move(remap));
+  return x ? Py_NewRef(a[9]) : THPVariable_Wrap(std::move(remap));
   END_HANDLE_TH_ERRORS
 }
 

@@ -6,10 +6,10 @@
 // Bound by the gather of the pages' rows: 580 bytes a page and query position, an SM's share of the measured copy rate is a tile (128 pages,
 // 74 KB) in 1.7 us, and its 18 MMAs of 128 x 128 x 32 take 0.9.  64 requests of 2048 pages, 128 heads: 24 us behind other kernels, of
 // which 6 are the first two tiles and the queries (4.3 TB/s from all SMs at once), 1.7 their conversion, then 2.6 a tile (4.2 TB/s); a
-// kernel that does nothing but read the same rows by number takes 22.3.  So a CTA per SM walks a contiguous range of the tiles of all rows, in two stages of a
-// whole tile each: at least one tile is in flight whatever the other roles do.  Rows come by cp.async straight into the
-// 64-byte swizzle of the operand (576 = 9 x 64 without a rest; eight rows x 64 bytes per instruction are one swizzle atom: no bank
-// conflicts, whole sectors); a TMA gather would take 288 instructions of 256 bytes a tile.
+// kernel that does nothing but read the same rows by number takes 22.3.  So a CTA per SM walks a contiguous range of the tiles of all
+// rows, in two stages of a whole tile each: at least one tile is in flight whatever the other roles do.  Rows come by cp.async straight into the
+// 64-byte swizzle of the operand (576 = 9 x 64 without a rest), 512 contiguous bytes an instruction; a TMA gather would take 288 instructions of
+// 256 bytes a tile.
 //
 // Few rows of one tile each (score_kernel<true>): a CTA has a row to itself, keeps its keys in shared memory and selects too, by counting for each page
 // those before it: no second launch, and nothing that another CTA has to see.

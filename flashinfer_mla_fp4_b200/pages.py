@@ -86,7 +86,8 @@ class FP4MLAPagePool:
 
     def _native(self, what: int, block_tables, seq_lens, x, y=None):
         """The common form of a call, checked and launched natively; None: nothing was done."""
-        return _cabi.native.pool(what, C.addressof(self._array), len(self._array), self.page_size, self.refcounts, self._status, block_tables, seq_lens, x, y)
+        return _cabi.native.pool(what, C.addressof(self._array), len(self._array), self.page_size, self.num_pages, self.refcounts, self._status,
+                                  block_tables, seq_lens, x, y)
 
     def num_free(self) -> int:
         """Free pages (synchronises)."""

@@ -235,3 +235,7 @@ def test_pool_refuses():
                  lambda: pool.compact(bt, sl, torch.empty(7, dtype=torch.int32, device=_dev()))):
         with pytest.raises(ValueError):
             call()
+    for wrong in (torch.zeros(9, dtype=torch.int32, device=_dev()), torch.zeros(7, dtype=torch.int32, device=_dev()), torch.zeros(8, device=_dev())):
+        pool.refcounts = wrong
+        with pytest.raises(ValueError, match="refcounts"):
+            pool.allocate(bt, sl, _i32([1, 1]))
