@@ -8,8 +8,7 @@
 // which 6 are the first two tiles and the queries (4.3 TB/s from all SMs at once), 1.7 their conversion, then 2.6 a tile (4.2 TB/s); a
 // kernel that does nothing but read the same rows by number takes 22.3.  So a CTA per SM walks a contiguous range of the tiles of all
 // rows, in two stages of a whole tile each: at least one tile is in flight whatever the other roles do.  Rows come by cp.async straight into the
-// 64-byte swizzle of the operand (576 = 9 x 64 without a rest), 512 contiguous bytes an instruction; a TMA gather would take 288 instructions of
-// 256 bytes a tile.
+// swizzled operand, 512 contiguous bytes an instruction; a TMA gather would take 160 instructions a tile.
 //
 // Few rows of one tile each (score_kernel<true>): a CTA has a row to itself, keeps its keys in shared memory and selects too, by counting for each page
 // those before it: no second launch, and nothing that another CTA has to see.
@@ -30,15 +29,14 @@ constexpr int kEpiWarps = 4, kLoadWarps = 8;
 constexpr int kMmaWarp = kEpiWarps, kFirstLoad = kEpiWarps + 1;
 constexpr int kThreads = 32 * (kEpiWarps + 1 + kLoadWarps);
 constexpr int kPages = 128;                       // pages of a tile: the lanes of TMEM
-constexpr int kBlocks = kQDim / 64;               // 64-byte blocks of a row: of the operands' swizzle
-constexpr int kChunks = kQDim / 16;               // 16-byte chunks
-constexpr int kStageBytes = kPages * kQDim;       // [9 blocks][128 pages][64 bytes], 64-byte swizzle
+static_assert(kQDim / 16 == 36, "a row is 32 chunks of 16 bytes and four more");
+constexpr int kStageBytes = kPages * kQDim;       // an operand of 128 pages (below)
 constexpr int kStages = 2;
 constexpr int kMaxRows = 1024;                    // rows of a launch (the launcher makes several)
 constexpr uint32_t kTmemCols = 256;               // two accumulators of up to 128 columns
 constexpr int kWholeKeys = kPages;                // most candidates of a row that a CTA has to itself
 
-// shared memory, from a 1024-byte boundary on: the stages, the query's codes [9][columns][64 bytes], then
+// shared memory, from a 1024-byte boundary on: the stages, the query's codes, then
 struct Small {
   int candidates[kMaxRows];  // pages that a row scores
   alignas(16) uint32_t keys[kWholeKeys];  // of a row that the CTA has to itself
@@ -78,10 +76,10 @@ struct Walk {
     while (candidates[r] == 0) ++r;
     return r;
   }
-  __device__ __forceinline__ void next() {
-    --left;
+  __device__ __forceinline__ void next() {  // (behind the last one there is none, however often)
+    if (--left <= 0) return;
     if (!row_ends()) ++tile;
-    else if (left > 0) row = next_row(), tile = 0;
+    else row = next_row(), tile = 0;
   }
   // block-table entry of page i of the tile, -1 where there is none
   __device__ __forceinline__ int entry(const SelectParams& p, int row0, int i) const {
@@ -94,30 +92,40 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// an arrival on the barrier once all copies that this thread has asked for have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
 
-// The 16-byte chunks of a warp's `rows` consecutive rows of 576 bytes, 32 at a time in the order of their addresses: f(row, chunk of it).
-struct Chunks {
-  int row = 0, chunk = threadIdx.x & 31;
-  __device__ __forceinline__ void next() {
-    chunk += 32;
-    const bool over = chunk >= kChunks;
-    chunk -= over ? kChunks : 0;
-    row += over;
+// An operand of `rows` rows: four blocks [rows][128 bytes] with the 128-byte swizzle, then one [rows][64 bytes] with the 64-byte swizzle.  (All in blocks of 64
+// bytes, eight lanes that store next to one another met in the same banks, and the stores took as long as the MMAs' reads.)
+__device__ __forceinline__ uint32_t wide_at(int rows, int row, int chunk) { return uint32_t((chunk >> 3) * (rows * 128) + row * 128 + (((chunk ^ row) & 7) << 4)); }
+__device__ __forceinline__ uint32_t tail_at(int rows, int row, int chunk) { return uint32_t(rows * 512 + row * 64 + (((chunk ^ (row >> 1)) & 3) << 4)); }
+// Rows `first` to `first + count - 1` of an operand, by a warp: 32 of a row's 36 chunks at a time, a lane each, then the last four of eight rows at a
+// time.  src(r): where row first + r comes from, asked by all lanes at once; null: nowhere.  (With the 32 next chunks in the order of their addresses,
+// whatever rows they belong to, the instructions that found their places took 4900 clk a tile, whether or not anything was loaded.)
+template <typename Src>
+__device__ __forceinline__ void copy_rows(uint32_t operand, int rows, int first, int count, Src src) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int r = 0; r < kPages / kLoadWarps; ++r) {
+    if (r >= count) break;
+    const char* from = src(r);
+    if (from) cp_async16(operand + wide_at(rows, first + r, lane), from + 16 * lane);
   }
-};
-template <typename F>
-__device__ __forceinline__ void for_chunks(int rows, F f) {
-#pragma unroll 3
-  for (Chunks c; c.row < rows; c.next()) f(c.row, c.chunk);
-}
-// where a chunk of a row lies in an operand of `rows` rows: [9 blocks][rows][64 bytes], 64-byte swizzle
-__device__ __forceinline__ uint32_t operand_at(int rows, int row, int chunk) {
-  return uint32_t((chunk >> 2) * (rows * 64) + row * 64 + (((chunk & 3) ^ ((row >> 1) & 3)) << 4));
+#pragma unroll
+  for (int h = 0; h < kPages / kLoadWarps; h += 8) {
+    const int r = h + (lane >> 2);
+    if (h >= count) break;
+    const char* from = src(r);
+    if (from && r < count) cp_async16(operand + tail_at(rows, first + r, lane), from + 16 * (32 + (lane & 3)));
+  }
 }
 
 // The heads of a row's query, to be the B operand: first fetched as they are, ...  Columns behind the last head repeat head 0, which leaves the
@@ -125,34 +133,36 @@ __device__ __forceinline__ uint32_t operand_at(int rows, int row, int chunk) {
 __device__ __forceinline__ void fetch_b(const SelectParams& p, uint32_t b_smem, int row, int columns) {
   const int each = columns / kLoadWarps, first = ((threadIdx.x >> 5) - kFirstLoad) * each, batch = row / p.q_len;
   const uint8_t* q = p.q + batch * p.q_stride_batch + (row - batch * p.q_len) * p.q_stride_qpos;
-  for_chunks(each, [&](int r, int chunk) {
+  copy_rows(b_smem, columns, first, each, [&](int r) {
     const int head = first + r;
-    cp_async16(b_smem + operand_at(columns, head, chunk), q + int64_t(head < p.heads ? head : 0) * p.q_stride_head + 16 * chunk);
+    return reinterpret_cast<const char*>(q + (head < p.heads ? head : 0) * p.q_stride_head);
   });
 }
-// ... then turned into integers where they lie: four lanes a head, eight heads at a time (a swizzle atom per access: no bank conflicts).  In FP16: an
-// E4M3 value times 2^k is exact, and adding 1536 rounds it to a whole number (to even, as round() does) that is the low byte of the sum.
+// ... then turned into integers where they lie: eight lanes a head, four heads at a time.  In FP16: an E4M3 value times 2^k is exact, and adding 1536
+// rounds it to a whole number (to even, as round() does) that is the low byte of the sum.
 __device__ __forceinline__ void convert_b(char* b_smem, float* unit, int columns) {
-  const int each = columns / kLoadWarps, first = ((threadIdx.x >> 5) - kFirstLoad) * each, lane = threadIdx.x & 31;
+  constexpr int kMine = 5;  // chunks of a lane; the last one of lanes 0-3 alone
+  const int each = columns / kLoadWarps, first = ((threadIdx.x >> 5) - kFirstLoad) * each, lane = threadIdx.x & 31, part = lane & 7;
 #pragma unroll 1
-  for (int r = lane >> 2; r < (each + 7) / 8 * 8; r += 8) {
+  for (int r = lane >> 3; r < (each + 3) / 4 * 4; r += 4) {
     const int head = first + (r < each ? r : 0);
-    uint4 v[kBlocks];
-    // the largest magnitude: bytes without their signs, by 16 bits; NaN is 127
-    uint32_t top = 0;
+    auto at = [&](int i) { return reinterpret_cast<uint4*>(b_smem + (i < 4 ? wide_at(columns, head, 8 * i + part) : tail_at(columns, head, part))); };
+    uint4 v[kMine];
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) v[i] = *reinterpret_cast<const uint4*>(b_smem + operand_at(columns, head, 4 * i + (lane & 3)));
+    for (int i = 0; i < kMine; ++i) v[i] = i < 4 || part < 4 ? *at(i) : make_uint4(0, 0, 0, 0);
+    // the largest magnitude: bytes without their signs, by 16 bits; NaN is 127
     auto top_of = [](const uint4& x) {
       const uint32_t a = __vmaxu2(x.x & 0x7f007f, x.y & 0x7f007f), b = __vmaxu2(x.z & 0x7f007f, x.w & 0x7f007f);
       const uint32_t c = __vmaxu2((x.x >> 8) & 0x7f007f, (x.y >> 8) & 0x7f007f), d = __vmaxu2((x.z >> 8) & 0x7f007f, (x.w >> 8) & 0x7f007f);
       return __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d));
     };
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) top = __vmaxu2(top, top_of(v[i]));
+    for (int i = 0; i < kMine; ++i) top = __vmaxu2(top, top_of(v[i]));
     if ((top & 0xffff) == 0x7f || top >> 16 == 0x7f) {  // NaN among them: they count as zero
       top = 0;
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
+      for (int i = 0; i < kMine; ++i) {
         uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -165,20 +175,20 @@ __device__ __forceinline__ void convert_b(char* b_smem, float* unit, int columns
     }
     __syncwarp();
     uint32_t most = max(top & 0xffff, top >> 16);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     const int binade = max(int(most >> 3), 1);  // exponent field
     const uint32_t half = uint32_t(15 + 13 - binade) << 10, times = half | half << 16;  // 2^(13 - binade)
     if (r >= each) continue;
-    if ((lane & 3) == 0) unit[head] = __uint_as_float(uint32_t(127 + binade - 13) << 23);
+    if (part == 0) unit[head] = __uint_as_float(uint32_t(127 + binade - 13) << 23);
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
+    for (int i = 0; i < kMine; ++i) {
       const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
       uint32_t out[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         out[j] = __byte_perm(hfma2(e4m3x2_to_f16x2(x[j] & 0xffff), times, 0x66006600u), hfma2(e4m3x2_to_f16x2(x[j] >> 16), times, 0x66006600u), 0x6420);
-      *reinterpret_cast<uint4*>(b_smem + operand_at(columns, head, 4 * i + (lane & 3))) = make_uint4(out[0], out[1], out[2], out[3]);
+      if (i < 4 || part < 4) *at(i) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
 }
@@ -231,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(bar(s.full_a[i]), kLoadWarps);
+      ptx::mbar_init(bar(s.full_a[i]), 32 * kLoadWarps);
       ptx::mbar_init(bar(s.empty_a[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -307,8 +317,11 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       // A row's query is fetched once the MMAs of the row before are over, which is known where the tile behind its first one is loaded.
       fetch_b(p, b_addr, row0 + k.row, columns);
       asm volatile("cp.async.commit_group;" ::: "memory");
-      // Page numbers come a tile ahead of their use, asked for before the rows of the tile before: behind those they would take as long.
-      int next_page = lane < kMine ? k.entry(p, row0, first + lane) : -1;
+      // Page numbers are asked for two tiles ahead, and before the rows: behind those they would take as long.
+      Walk ahead(s);
+      int pages[2];  // of the next two tiles
+#pragma unroll
+      for (int i = 0; i < 2; ++i, ahead.next()) pages[i] = lane < kMine ? ahead.entry(p, row0, first + lane) : -1;
       int fresh = -1, seg = 0;  // fresh: the row that the last tile was the first of, or -1
       bool ok = true;
       for (int n = 0; ; ++n) {
@@ -323,30 +336,27 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         const int next_fresh = more && (n == 0 || k.tile == 0) ? k.row : -1;
         if (more) {
           k.next();
-          const int page = next_page < p.num_pages ? next_page : -1;
-          next_page = lane < kMine ? k.entry(p, row0, first + lane) : -1;
+          const int page = pages[0] < p.num_pages ? pages[0] : -1;
+          pages[0] = pages[1];
+          pages[1] = lane < kMine ? ahead.entry(p, row0, first + lane) : -1;
+          ahead.next();
           // (rows without a page are left as they are: what comes of them nobody reads.  With some page in their place, the same for all, the tiles
           // that are not full had all SMs wait for one line: 148 rows of 57 candidates 21.2 us instead of 11.5.)
-          for_chunks(kMine, [&](int r, int chunk) {
+          copy_rows(a_addr + st * kStageBytes, kPages, first, kMine, [&](int r) {
             const int from = __shfl_sync(0xffffffffu, page, r);
-            if (from >= 0) cp_async16(a_addr + st * kStageBytes + operand_at(kPages, first + r, chunk), p.summary + int64_t(from) * kQDim + 16 * chunk);
+            return from >= 0 ? reinterpret_cast<const char*>(p.summary + int64_t(from) * kQDim) : nullptr;
           });
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (n > 0) {
-          if (fresh >= 0) {
-            if (seg == 0) asm volatile("cp.async.wait_group 2;" ::: "memory");  // the query came first, both tiles may still be on their way
-            else asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncwarp();  // (a lane converts what others have fetched)
-            convert_b(b_smem, s.unit[seg++ & 3], columns);
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(bar(s.full_b));
-          }
-          asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the tile just asked for
+        if (more) cp_async_arrive(bar(s.full_a[st]));  // (nobody waits here for a tile: its MMAs start when it is there)
+        if (n > 0 && fresh >= 0) {
+          if (seg == 0) asm volatile("cp.async.wait_group 2;" ::: "memory");  // the query came first, both tiles may still be on their way
+          else asm volatile("cp.async.wait_group 1;" ::: "memory");
+          __syncwarp();  // (a lane converts what others have fetched)
+          convert_b(b_smem, s.unit[seg++ & 3], columns);
           ptx::fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(s.full_a[st ^ 1]));
+          if (lane == 0) ptx::mbar_arrive(bar(s.full_b));
         }
         fresh = next_fresh;
         if (!more) break;
@@ -355,7 +365,8 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
     } else if (warp == kMmaWarp) {
       // ------------------------------------------------------------------ MMAs
       const uint32_t e = ptx::elect_one();
-      const uint64_t a0 = ptx::smem_desc(ptx::smem_u32(a_smem), 16, 512, 4), b0 = ptx::smem_desc(ptx::smem_u32(b_smem), 16, 512, 4);
+      const uint64_t a0 = ptx::smem_desc(ptx::smem_u32(a_smem), 16, 1024, 2), b0 = ptx::smem_desc(ptx::smem_u32(b_smem), 16, 1024, 2);
+      const uint64_t a4 = ptx::smem_desc(ptx::smem_u32(a_smem) + kPages * 512, 16, 512, 4), b4 = ptx::smem_desc(ptx::smem_u32(b_smem) + columns * 512, 16, 512, 4);
       // D: S32; A, B: signed 8-bit, K-major
       const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(columns >> 3) << 17) | (uint32_t(kPages >> 4) << 24);
       int seg = 0;
@@ -367,11 +378,14 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         if (ok && n >= 2) ok = wait(c, s.empty_d[st], ((n >> 1) - 1) & 1);
         if (ok) ok = wait(c, s.full_a[st], (n >> 1) & 1);
         if (!ok) break;
+        ptx::fence_proxy_async_smem();  // the copies into the stage were not the async proxy's; the MMAs' reads are
         ptx::tc_fence_after();
 #pragma unroll
-        for (uint32_t i = 0; i < kQDim / 32; ++i)
-          ptx::umma_i8(e, tmem + st * 128, a0 + ((st * kStageBytes + (i >> 1) * (kPages * 64)) >> 4) + 2 * (i & 1),
-                       b0 + (((i >> 1) * (columns * 64)) >> 4) + 2 * (i & 1), idesc, i);
+        for (uint32_t i = 0; i < 16; ++i)
+          ptx::umma_i8(e, tmem + st * 128, a0 + ((st * kStageBytes + (i >> 2) * (kPages * 128)) >> 4) + 2 * (i & 3),
+                       b0 + (((i >> 2) * (columns * 128)) >> 4) + 2 * (i & 3), idesc, i);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) ptx::umma_i8(e, tmem + st * 128, a4 + ((st * kStageBytes) >> 4) + 2 * i, b4 + 2 * i, idesc, 1u);
         if (e) ptx::umma_commit(bar(s.empty_a[st]));
         if (e) {
           ptx::umma_commit(bar(s.full_d[st]));
@@ -388,14 +402,27 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       __syncwarp();
     } else {
       // ------------------------------------------------------------------ scores
-      Walk k(s);
-      int seg = 0, next_page = k.entry(p, row0, tid);
+      // A page's number is asked for three tiles ahead and its scale two: with everybody loading they take longer than a tile (asked for with the
+      // tile before they made an epilogue of 4800 clk of one of 1400).
+      Walk k(s), ahead(s);
+      auto scale_of = [&](int page) { return page >= 0 && page < p.num_pages ? __ldcg(p.summary_sf + page) : 0.f; };
+      int seg = 0, pages[3];
+      float scales[2];
+#pragma unroll
+      for (int i = 0; i < 3; ++i, ahead.next()) pages[i] = ahead.entry(p, row0, tid);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) scales[i] = scale_of(pages[i]);
       for (int n = 0; k.left > 0; ++n) {
-        const int st = n & 1, row = k.row, i = k.tile * kPages + tid, page = next_page;
+        const int st = n & 1, row = k.row, i = k.tile * kPages + tid, page = pages[0];
         const bool scored = i < k.candidates[row], last = k.row_ends(), there = page >= 0 && page < p.num_pages;
-        const float scale = there ? __ldcg(p.summary_sf + page) : 0.f;
+        const float scale = scales[0];
         k.next();
-        next_page = k.entry(p, row0, tid);
+        pages[0] = pages[1];
+        pages[1] = pages[2];
+        pages[2] = ahead.entry(p, row0, tid);
+        ahead.next();
+        scales[0] = scales[1];
+        scales[1] = scale_of(pages[1]);
         if (!wait(c, s.full_d[st], (n >> 1) & 1)) break;
         const float* unit = s.unit[seg & 3];
         ptx::tc_fence_after();
