@@ -113,16 +113,14 @@ __device__ __forceinline__ uint32_t tail_at(int rows, int row, int chunk) { retu
 template <typename Src>
 __device__ __forceinline__ void copy_rows(uint32_t operand, int rows, int first, int count, Src src) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int r = 0; r < kPages / kLoadWarps; ++r) {
-    if (r >= count) break;
+#pragma unroll 4
+  for (int r = 0; r < count; ++r) {
     const char* from = src(r);
     if (from) cp_async16(operand + wide_at(rows, first + r, lane), from + 16 * lane);
   }
-#pragma unroll
-  for (int h = 0; h < kPages / kLoadWarps; h += 8) {
+#pragma unroll 1
+  for (int h = 0; h < count; h += 8) {
     const int r = h + (lane >> 2);
-    if (h >= count) break;
     const char* from = src(r);
     if (from && r < count) cp_async16(operand + tail_at(rows, first + r, lane), from + 16 * (32 + (lane & 3)));
   }
