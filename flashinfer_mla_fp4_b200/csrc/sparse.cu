@@ -279,15 +279,19 @@ __global__ void __launch_bounds__(kSumThreads) summarize_four_kernel(SummarizePa
 // ------------------------------------------------------------------------------------------ selection
 // A CTA per row.  A thread has kKeys consecutive keys in registers (and their block-table entries: all loads of a row are on their way at once,
 // before its length is known).  The key of the last page that is taken is found by counting the keys' range in 256 buckets, going on with the
-// bucket in which the count reaches what is wanted: two rounds where keys are spread, four where they are not or pages tie.
-// Then one scan gives each page that is taken its place.  64 rows of 2048 pages, nothing in L2: 39.8 us by bytes of the keys, whose leading
-// byte is nearly everybody's, so that all threads wanted the same counter; 9.8 by halving the range with a barrier each time; 6.7 so.
+// bucket in which the count reaches what is wanted until it holds so few that they are compared with one another: one round where keys
+// are spread.  A page's place in the order is its key and, below that, its index from the last one: pages that tie have places of their own.
+// Then one scan gives each page that is taken its place in the table.  64 rows of 2048 pages, nothing in L2: 39.8 us by bytes of the keys, whose leading
+// byte is nearly everybody's, so that all threads wanted the same counter; 9.8 by halving the range with a barrier each time; 6.7 by buckets down to
+// a single key; 5.6 so, of which 1.5 are loads, 0.8 a round, 0.7 the comparing, 0.4 the scan.
 // kKeys = 0: more candidates than registers hold; the keys stay in global memory and are read through L2 in each round.
-constexpr int kSelMost = 1024, kBuckets = 256;
+constexpr int kSelMost = 1024, kBuckets = 256, kList = 128;
 
 template <int kKeys>
 __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
-  __shared__ uint32_t range_s[2][32], bucket_s[kBuckets], found_s[3];
+  __shared__ uint32_t range_s[2][32], found_s[3], listed_s;
+  __shared__ alignas(16) uint32_t bucket_s[kBuckets];
+  __shared__ uint64_t list_s[kList], least_s;
   dependent_launch();
   const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
   const uint32_t* keys = p.keys + int64_t(row) * p.key_stride;
@@ -311,119 +315,157 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
         for (int j = i; j < i + 4; ++j) page[j] = p.sink + tid * kKeys + j < p.width ? __ldcg(table + p.sink + tid * kKeys + j) : 0;
     }
   }
+  for (int k = tid; k < kBuckets; k += blockDim.x) bucket_s[k] = 0;
+  if (tid == 0) listed_s = 0;
   const Seen v = seen(p, row);
   if (v.used <= p.budget) {  // the budget holds them all
     for (int k = tid; k < p.budget; k += blockDim.x) out[k] = k < v.used ? __ldcg(table + k) : 0;
     if (tid == 0) p.selected_lens[row] = v.len;
     return;
   }
-  const int candidates = v.used - p.sink - p.local, wanted = p.budget - p.sink - p.local;
+  const int edges = p.sink + p.local, candidates = v.used - edges, wanted = p.budget - edges;
+  // the sink and the local pages: a thread's first one is asked for here and stored at the end
+  auto edge_of = [&](int k) { return __ldcg(table + (k < p.sink ? k : v.used - edges + k)); };
+  auto store_edge = [&](int k, int32_t page) { out[k < p.sink ? k : p.budget - edges + k] = page; };
+  const int32_t edge = tid < edges ? edge_of(tid) : 0;
   const int mine = kKeys ? kKeys : (candidates + int(blockDim.x) - 1) / int(blockDim.x);
   const int first = tid * mine, last = min(first + mine, candidates);
-  auto for_keys = [&](auto f) {  // f(key, its page when called)
+  // f(key of a candidate, its index, i: which of this thread's)
+  auto for_keys = [&](auto f) {
     if constexpr (kKeys > 0) {
 #pragma unroll
       for (int i = 0; i < kKeys; ++i)
-        if (first + i < candidates) f(reg[i], [&] { return kPagesToo ? page[kPagesToo ? i : 0] : __ldcg(table + p.sink + first + i); });
+        if (first + i < candidates) f(reg[i], first + i, i);
     } else {
-      for (int k = first; k < last; ++k) f(__ldcg(keys + k), [&] { return __ldcg(table + p.sink + k); });
+      for (int k = first; k < last; ++k) f(__ldcg(keys + k), k, k - first);
     }
   };
-  for (int k = tid; k < p.sink; k += blockDim.x) out[k] = __ldcg(table + k);
-  for (int k = tid; k < p.local; k += blockDim.x) out[p.budget - p.local + k] = __ldcg(table + v.used - p.local + k);
-  if (tid == 0) p.selected_lens[row] = v.len - (v.used - p.budget) * p.page_size;
-  if (wanted == 0) return;
-  uint32_t low = 0xffffffffu, high = 0;
-  for_keys([&](uint32_t key, auto) {
-    low = min(low, key);
-    high = max(high, key);
-  });
-  low = __reduce_min_sync(0xffffffffu, low);
-  high = __reduce_max_sync(0xffffffffu, high);
-  if (lane == 0) {
-    range_s[0][warp] = low;
-    range_s[1][warp] = high;
-  }
-  for (int k = tid; k < kBuckets; k += blockDim.x) bucket_s[k] = 0;
-  __syncthreads();
-  low = __reduce_min_sync(0xffffffffu, range_s[0][lane < warps ? lane : 0]);
-  high = __reduce_max_sync(0xffffffffu, range_s[1][lane < warps ? lane : 0]);
-  // Keys above `high` are fewer than wanted (none, to begin with), keys from `low` on are enough.
-  uint32_t above = 0;  // keys > high
-  while (low < high) {
-    const int shift = max(0, 24 - __clz(high - low));  // 256 buckets hold the range
-    for_keys([&](uint32_t key, auto) {
-      if (key >= low && key <= high) atomicAdd(&bucket_s[(key - low) >> shift], 1u);
-    });
+  auto place_of = [](uint32_t key, int k) { return uint64_t(key) << 32 | uint32_t(~k); };
+  // of this thread's count those of the threads before it, too; the last thread's is the sum
+  auto scan = [&](uint32_t count) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t down = __shfl_up_sync(0xffffffffu, count, o);
+      count += lane >= o ? down : 0;
+    }
+    if (lane == 31) range_s[0][warp] = count;
     __syncthreads();
-    if (warp == 0) {  // lane i has the buckets 8 i to 8 i + 7: the one, from above, in which the count reaches what is wanted
-      uint32_t n[8], sum = 0;
+    return count + __reduce_add_sync(0xffffffffu, lane < warp ? range_s[0][lane] : 0u);
+  };
+  if (wanted > 0) {
+    uint32_t low = 0xffffffffu, high = 0;
+    for_keys([&](uint32_t key, int, int) {
+      low = min(low, key);
+      high = max(high, key);
+    });
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0) {
+      range_s[0][warp] = low;
+      range_s[1][warp] = high;
+    }
+    __syncthreads();
+    low = __reduce_min_sync(0xffffffffu, range_s[0][lane < warps ? lane : 0]);
+    high = __reduce_max_sync(0xffffffffu, range_s[1][lane < warps ? lane : 0]);
+    // Keys above `high` are fewer than wanted (`above`; none, to begin with), keys from `low` on are enough; `within` lie from low to high.
+    uint32_t above = 0, within = candidates;
+    while (low < high && within > kList) {
+      const int shift = max(0, 24 - __clz(high - low));  // 256 buckets hold the range
+      for_keys([&](uint32_t key, int, int) {
+        if (key - low <= high - low) atomicAdd(&bucket_s[(key - low) >> shift], 1u);
+      });
+      __syncthreads();
+      if (warp == 0) {  // lane i has the buckets 8 i to 8 i + 7: the one, from above, in which the count reaches what is wanted
+        uint4* const eight = reinterpret_cast<uint4*>(bucket_s + 8 * lane);
+        const uint4 a = eight[0], b = eight[1];
+        eight[0] = eight[1] = make_uint4(0, 0, 0, 0);
+        const uint32_t n[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t sum = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        n[i] = bucket_s[8 * lane + i];
-        sum += n[i];
-        bucket_s[8 * lane + i] = 0;
-      }
-      uint32_t from = sum;  // of this lane and those above it
+        for (int i = 0; i < 8; ++i) sum += n[i];
+        uint32_t from = sum;  // of this lane and those above it
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t a = __shfl_down_sync(0xffffffffu, from, o);
-        from += lane + o < 32 ? a : 0;
-      }
-      uint32_t over = above + from - sum;
-      if (over < uint32_t(wanted) && over + sum >= uint32_t(wanted)) {
-        bool found = false;
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t up = __shfl_down_sync(0xffffffffu, from, o);
+          from += lane + o < 32 ? up : 0;
+        }
+        uint32_t over = above + from - sum;
+        if (over < uint32_t(wanted) && over + sum >= uint32_t(wanted)) {
 #pragma unroll
-        for (int i = 7; i >= 0; --i) {
-          if (!found && over + n[i] >= uint32_t(wanted)) {
-            found = true;
-            found_s[0] = 8 * lane + i;
-            found_s[1] = over;
-            found_s[2] = n[i];
+          for (int i = 7; i >= 0; --i) {
+            if (over < uint32_t(wanted) && over + n[i] >= uint32_t(wanted)) {
+              found_s[0] = 8 * lane + i;
+              found_s[1] = over;
+              found_s[2] = n[i];
+            }
+            over += n[i];
           }
-          over += n[i];
         }
       }
+      __syncthreads();
+      low += found_s[0] << shift;
+      above = found_s[1];
+      within = found_s[2];
+      high = low + min(high - low, (1u << shift) - 1);  // (the bucket's end may lie beyond 32 bits)
     }
-    __syncthreads();
-    const uint32_t bucket = found_s[0], start = low + (bucket << shift);
-    above = found_s[1];
-    if (above + found_s[2] == uint32_t(wanted)) {  // the whole bucket is taken: these are the ones
-      high = start - 1;
-      above = wanted;
-      break;
-    }
-    high = start + min(high - start, (1u << shift) - 1);  // (the bucket's end may lie beyond 32 bits)
-    low = start;
-  }
-  // taken: keys > high, and of those equal to it the first wanted - above
-  const uint32_t ties = uint32_t(wanted) - above;
-  uint32_t more = 0, equal = 0;
-  for_keys([&](uint32_t key, auto) {
-    more += key > high;
-    equal += key == high;
-  });
-  uint32_t more_before = more, equal_before = equal;
+    uint64_t least = place_of(low, -1);  // place of the last one that is taken, or below it
+    const uint32_t rest = wanted - above;
+    if (rest < within) {
+      if (within <= kList) {  // few enough to be compared with one another
+        uint32_t listed = 0;
+        for_keys([&](uint32_t key, int, int) { listed += key - low <= high - low; });
+        if (listed) {  // (one counter's answer a thread: an answer takes 200 clk)
+          uint64_t* next = list_s + atomicAdd(&listed_s, listed);
+          for_keys([&](uint32_t key, int k, int) {
+            if (key - low <= high - low) *next++ = place_of(key, k);
+          });
+        }
+        __syncthreads();
+        uint64_t some[kList / 32];  // a lane has up to four of them; a warp counts those before one of them at a time
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t a = __shfl_up_sync(0xffffffffu, more_before, o), b = __shfl_up_sync(0xffffffffu, equal_before, o);
-    more_before += lane >= o ? a : 0;
-    equal_before += lane >= o ? b : 0;
+        for (int i = 0; i < kList / 32; ++i) some[i] = lane + 32 * i < within ? list_s[lane + 32 * i] : 0;
+#pragma unroll 2
+        for (uint32_t k = warp; k < within; k += warps) {
+          const uint64_t place = list_s[k];
+          uint32_t before = 1;
+#pragma unroll
+          for (int i = 0; i < kList / 32; ++i) before += __popc(__ballot_sync(0xffffffffu, some[i] > place));
+          if (before == rest && lane == 0) least_s = place;
+        }
+      } else {  // all of one key: the first ones
+        uint32_t equal = 0;
+        for_keys([&](uint32_t key, int, int) { equal += key == low; });
+        uint32_t before = scan(equal) - equal;
+        for_keys([&](uint32_t key, int k, int) {
+          if (key == low && ++before == rest) least_s = place_of(key, k);
+        });
+      }
+      __syncthreads();
+      least = least_s;
+    }
+    // those from `least` on are taken, in the order of their indices
+    uint32_t taken = 0, which = 0;  // (which: kKeys > 0, as bits)
+    for_keys([&](uint32_t key, int k, int i) {
+      const bool take = place_of(key, k) >= least;
+      taken += take;
+      if constexpr (kKeys > 0) which |= uint32_t(take) << i;
+      if constexpr (kKeys > 0 && !kPagesToo)
+        if (take) reg[i] = uint32_t(__ldcg(table + p.sink + k));  // (on their way during the scan)
+    });
+    int32_t* next = out + p.sink + scan(taken) - taken;
+    if constexpr (kKeys > 0) {
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i)
+        if (which >> i & 1) *next++ = kPagesToo ? page[kPagesToo ? i : 0] : int32_t(reg[i]);
+    } else {
+      for_keys([&](uint32_t key, int k, int) {
+        if (place_of(key, k) >= least) *next++ = __ldcg(table + p.sink + k);
+      });
+    }
   }
-  __syncthreads();
-  if (lane == 31) {
-    range_s[0][warp] = more_before;
-    range_s[1][warp] = equal_before;
-  }
-  __syncthreads();
-  more_before += __reduce_add_sync(0xffffffffu, lane < warp ? range_s[0][lane] : 0u) - more;
-  equal_before += __reduce_add_sync(0xffffffffu, lane < warp ? range_s[1][lane] : 0u) - equal;
-  for_keys([&](uint32_t key, auto page_of) {
-    const bool tie = key == high;
-    if (key > high || (tie && equal_before < ties)) out[p.sink + more_before + min(equal_before, ties)] = page_of();
-    more_before += key > high;
-    equal_before += tie;
-  });
+  if (tid < edges) store_edge(tid, edge);
+  for (int k = tid + blockDim.x; k < edges; k += blockDim.x) store_edge(k, edge_of(k));
+  if (tid == 0) p.selected_lens[row] = v.len - (v.used - p.budget) * p.page_size;
 }
 
 }  // namespace
