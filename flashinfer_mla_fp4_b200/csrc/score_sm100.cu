@@ -312,7 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       const int first = (warp - kFirstLoad) * kMine;
       const uint32_t a_addr = ptx::smem_u32(a_smem), b_addr = ptx::smem_u32(b_smem);
       Walk k(s);
-      // A row's query is fetched once the MMAs of the row before are over, which is known where the tile behind its first one is loaded.
+      // A row's query is fetched once the MMAs of the row before are over, which is known where the tile behind its first one is loaded; the
+      // first row's before anything, and converted while the first tile is on its way (behind the second one: 24.4 us instead of 23.6 for 32 rows of
+      // 2048 pages).
       fetch_b(p, b_addr, row0 + k.row, columns);
       asm volatile("cp.async.commit_group;" ::: "memory");
       // Page numbers are asked for two tiles ahead, and before the rows: behind those they would take as long.
@@ -327,11 +329,11 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         const bool more = k.left > 0;
         if (n >= kStages && (more || fresh >= 0)) ok = wait(c, s.empty_a[st], ((n >> 1) - 1) & 1);
         if (!ok) break;
-        if (fresh >= 0 && seg > 0) {
+        if (fresh >= 0) {
           fetch_b(p, b_addr, row0 + fresh, columns);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        const int next_fresh = more && (n == 0 || k.tile == 0) ? k.row : -1;
+        const int next_fresh = more && n > 0 && k.tile == 0 ? k.row : -1;
         if (more) {
           k.next();
           const int page = pages[0] < p.num_pages ? pages[0] : -1;
@@ -347,9 +349,8 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (more) cp_async_arrive(bar(s.full_a[st]));  // (nobody waits here for a tile: its MMAs start when it is there)
-        if (n > 0 && fresh >= 0) {
-          if (seg == 0) asm volatile("cp.async.wait_group 2;" ::: "memory");  // the query came first, both tiles may still be on their way
-          else asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (n == 0 || fresh >= 0) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");  // the query came first, the tile may still be on its way
           __syncwarp();  // (a lane converts what others have fetched)
           convert_b(b_smem, s.unit[seg++ & 3], columns);
           ptx::fence_proxy_async_smem();
