@@ -4,17 +4,18 @@
 // largest over heads would be a reduction across threads, and fewer than 128 heads would waste half of the MMA or more.
 //
 // Bound by the gather of the pages' rows: 580 bytes a page and query position, an SM's share of the measured copy rate is a tile (128 pages,
-// 74 KB) in 1.7 us, and its 18 MMAs of 128 x 128 x 32 take 0.9.  64 requests of 2048 pages, 128 heads: 24 us behind other kernels, of
-// which 6 are the first two tiles and the queries (4.3 TB/s from all SMs at once), 1.7 their conversion, then 2.6 a tile (4.2 TB/s); a
-// kernel that does nothing but read the same rows by number takes 22.3.  So a CTA per SM walks a contiguous range of the tiles of all
-// rows, in two stages of a whole tile each: at least one tile is in flight whatever the other roles do.  Rows come by cp.async straight into the
-// swizzled operand, 512 contiguous bytes an instruction; a TMA gather would take 160 instructions a tile.
+// 74 KB) in 1.7 us, and its 18 MMAs of 128 x 128 x 32 take 0.9.  64 requests of 2048 pages, 128 heads, up to seven tiles a CTA: 18.5 us, of which 2.1 are
+// up to the CTA's share, 3.2 the query and the first tile, 1.9 the conversion, then 1.5 a tile (7 TB/s, some of it out of L2).  So a CTA per SM
+// walks a contiguous range of the tiles of all rows, in two stages of a whole tile each: at least one tile is in flight whatever the other roles do.
+// Rows come by cp.async straight into the swizzled operand, 512 contiguous bytes an instruction, 32 bytes a clk and SM; a TMA gather would
+// take 160 instructions a tile.
 //
 // Few rows of one tile each (score_kernel<true>): a CTA has a row to itself, keeps its keys in shared memory and selects too, by counting for each page
 // those before it: no second launch, and nothing that another CTA has to see.
 //
-// Roles: warps 0-3 take the scores out of TMEM, warp 4 issues the MMAs, warps 5-12 load, and turn a row's query into integers (the B
-// operand) while the row's first two tiles are on their way.  All waits are bounded; one that runs out sets the status and ends the CTA, whose
+// Roles: warps 0-3 take the scores out of TMEM, warp 4 issues the MMAs, warps 5-20 load, and turn a row's query into integers (the B
+// operand) while the row's first tile is on its way.  (With eight warps for that instead of sixteen 32 requests of 2048 pages, 128 heads, with their
+// attention took 67.7 us instead of 66.0, 64 such selections 28.1 instead of 27.2; one of 16 heads 7.6 instead of 8.0.)  All waits are bounded; one that runs out sets the status and ends the CTA, whose
 // keys are then not all written.
 #include "common.cuh"
 #include "launch.h"
@@ -25,7 +26,7 @@ namespace mla {
 
 namespace {
 
-constexpr int kEpiWarps = 4, kLoadWarps = 8;
+constexpr int kEpiWarps = 4, kLoadWarps = 16;
 constexpr int kMmaWarp = kEpiWarps, kFirstLoad = kEpiWarps + 1;
 constexpr int kThreads = 32 * (kEpiWarps + 1 + kLoadWarps);
 constexpr int kPages = 128;                       // pages of a tile: the lanes of TMEM
@@ -39,6 +40,7 @@ constexpr int kWholeKeys = kPages;                // most candidates of a row th
 // shared memory, from a 1024-byte boundary on: the stages, the query's codes, then
 struct Small {
   int candidates[kMaxRows];  // pages that a row scores
+  uint16_t request[kMaxRows];  // of a row, counted from the first row's (a division at every tile's page numbers: 1 us for 15 rows of 3750 pages)
   alignas(16) uint32_t keys[kWholeKeys];  // of a row that the CTA has to itself
   int taken[kWholeKeys / 32];
   float unit[4][128];        // 2^-k of the heads, by row: an epilogue may be three tiles, so three rows, behind the loads
@@ -68,8 +70,9 @@ __device__ __forceinline__ bool wait(const Ctx& c, const unsigned long long& b, 
 // The tiles of a CTA in order, the same for every role.
 struct Walk {
   const int* candidates;
+  const uint16_t* request;
   int row, tile, left;
-  __device__ __forceinline__ Walk(const Small& s) : candidates(s.candidates), row(s.first_row), tile(s.first_tile), left(s.tiles) {}
+  __device__ __forceinline__ Walk(const Small& s) : candidates(s.candidates), request(s.request), row(s.first_row), tile(s.first_tile), left(s.tiles) {}
   __device__ __forceinline__ bool row_ends() const { return (tile + 1) * kPages >= candidates[row]; }
   __device__ __forceinline__ int next_row() const {  // (there is one where tiles are left)
     int r = row + 1;
@@ -82,9 +85,9 @@ struct Walk {
     else row = next_row(), tile = 0;
   }
   // block-table entry of page i of the tile, -1 where there is none
-  __device__ __forceinline__ int entry(const SelectParams& p, int row0, int i) const {
+  __device__ __forceinline__ int entry(const SelectParams& p, const int32_t* tables, int i) const {
     i += tile * kPages;
-    return left > 0 && i < candidates[row] ? __ldcg(p.block_tables + int64_t((row0 + row) / p.q_len) * p.block_table_stride + p.sink + i) : -1;
+    return left > 0 && i < candidates[row] ? __ldcg(tables + int64_t(request[row]) * p.block_table_stride + i) : -1;
   }
 };
 
@@ -257,24 +260,28 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if constexpr (kWhole) row0 = blockIdx.x;
+  const int request0 = row0 / p.q_len;
+  const int32_t* const tables = p.block_tables + int64_t(request0) * p.block_table_stride + p.sink;  // of the first row's request, its candidates
   Seen mine{0, 0};
   int page_of_mine = 0;  // of the candidate that this thread may take
   if constexpr (kWhole) {
-    row0 = blockIdx.x;
     mine = seen(p, row0);
     const int candidates = mine.used > p.budget ? mine.used - p.sink - p.local : 0;
     if (tid == 0) {
       s.candidates[0] = candidates;
+      s.request[0] = 0;
       s.first_row = s.first_tile = 0;
       s.tiles = (candidates + kPages - 1) / kPages;
     }
     if (tid < kWholeKeys) {
       s.keys[tid] = 0;
-      if (tid < candidates) page_of_mine = __ldcg(p.block_tables + int64_t(row0 / p.q_len) * p.block_table_stride + p.sink + tid);
+      if (tid < candidates) page_of_mine = __ldcg(tables + tid);
     }
   } else {
     for (int r = tid; r < rows; r += kThreads) {
       const Seen v = seen(p, row0 + r);
+      s.request[r] = uint16_t((row0 + r) / p.q_len - request0);
       s.candidates[r] = v.used > p.budget ? v.used - p.sink - p.local : 0;
     }
   }
@@ -321,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       Walk ahead(s);
       int pages[2];  // of the next two tiles
 #pragma unroll
-      for (int i = 0; i < 2; ++i, ahead.next()) pages[i] = lane < kMine ? ahead.entry(p, row0, first + lane) : -1;
+      for (int i = 0; i < 2; ++i, ahead.next()) pages[i] = lane < kMine ? ahead.entry(p, tables, first + lane) : -1;
       int fresh = -1, seg = 0;  // fresh: the row that the last tile was the first of, or -1
       bool ok = true;
       for (int n = 0; ; ++n) {
@@ -338,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
           k.next();
           const int page = pages[0] < p.num_pages ? pages[0] : -1;
           pages[0] = pages[1];
-          pages[1] = lane < kMine ? ahead.entry(p, row0, first + lane) : -1;
+          pages[1] = lane < kMine ? ahead.entry(p, tables, first + lane) : -1;
           ahead.next();
           // (rows without a page are left as they are: what comes of them nobody reads.  With some page in their place, the same for all, the tiles
           // that are not full had all SMs wait for one line: 148 rows of 57 candidates 21.2 us instead of 11.5.)
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       int seg = 0, pages[3];
       float scales[2];
 #pragma unroll
-      for (int i = 0; i < 3; ++i, ahead.next()) pages[i] = ahead.entry(p, row0, tid);
+      for (int i = 0; i < 3; ++i, ahead.next()) pages[i] = ahead.entry(p, tables, tid);
 #pragma unroll
       for (int i = 0; i < 2; ++i) scales[i] = scale_of(pages[i]);
       for (int n = 0; k.left > 0; ++n) {
@@ -418,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         k.next();
         pages[0] = pages[1];
         pages[1] = pages[2];
-        pages[2] = ahead.entry(p, row0, tid);
+        pages[2] = ahead.entry(p, tables, tid);
         ahead.next();
         scales[0] = scales[1];
         scales[1] = scale_of(pages[1]);
