@@ -151,15 +151,15 @@ __device__ __forceinline__ void convert_b(char* b_smem, float* unit, int columns
     uint4 v[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) v[i] = i < 4 || part < 4 ? *at(i) : make_uint4(0, 0, 0, 0);
-    // the largest magnitude: bytes without their signs, by 16 bits; NaN is 127
-    auto top_of = [](const uint4& x) {
-      const uint32_t a = __vmaxu2(x.x & 0x7f007f, x.y & 0x7f007f), b = __vmaxu2(x.z & 0x7f007f, x.w & 0x7f007f);
-      const uint32_t c = __vmaxu2((x.x >> 8) & 0x7f007f, (x.y >> 8) & 0x7f007f), d = __vmaxu2((x.z >> 8) & 0x7f007f, (x.w >> 8) & 0x7f007f);
-      return __vmaxu2(__vmaxu2(a, b), __vmaxu2(c, d));
+    // the largest magnitude: bytes without their signs, by 16 bits, the upper ones with what lies below them; NaN is 127
+    auto top_of = [](uint32_t top, const uint4& x) {
+      const uint32_t a = __vmaxu2(x.x & 0x7fff7fff, x.y & 0x7fff7fff), b = __vmaxu2(x.z & 0x7fff7fff, x.w & 0x7fff7fff);
+      const uint32_t c = __vmaxu2(x.x & 0x7f007f, x.y & 0x7f007f), d = __vmaxu2(x.z & 0x7f007f, x.w & 0x7f007f);
+      return __vmaxu2(__vmaxu2(top, __vmaxu2(a, b) >> 8 & 0x7f007f), __vmaxu2(c, d));
     };
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) top = __vmaxu2(top, top_of(v[i]));
+    for (int i = 0; i < kMine; ++i) top = top_of(top, v[i]);
     if ((top & 0xffff) == 0x7f || top >> 16 == 0x7f) {  // NaN among them: they count as zero
       top = 0;
 #pragma unroll
@@ -171,7 +171,7 @@ __device__ __forceinline__ void convert_b(char* b_smem, float* unit, int columns
           x[j] &= ~(nan | (nan - (nan >> 7)));
         }
         v[i] = make_uint4(x[0], x[1], x[2], x[3]);
-        top = __vmaxu2(top, top_of(v[i]));
+        top = top_of(top, v[i]);
       }
     }
     __syncwarp();
@@ -289,17 +289,18 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = s.tmem;
-  if (!kWhole && warp == 0) {  // this CTA's share: tiles [T i / n, T (i + 1) / n) of all tiles in the order of the rows
-    long long total = 0;
+  if (!kWhole && warp == 0) {  // this CTA's share of all tiles in the order of the rows
+    uint32_t total = 0;  // (at most 2^10 rows of 2^31 tokens: 2^31 tiles of 128 pages of 8)
     for (int base = 0; base < rows; base += 32)
       total += __reduce_add_sync(0xffffffffu, base + lane < rows ? (s.candidates[base + lane] + kPages - 1) / kPages : 0);
-    const long long lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
-    long long at = 0;
+    const uint32_t each = total / gridDim.x, rest = total - each * gridDim.x;
+    const uint32_t lo = each * blockIdx.x + min(blockIdx.x, rest), hi = lo + each + (blockIdx.x < rest);
+    uint32_t at = 0;
     for (int base = 0; base < rows && at <= lo && hi > lo; base += 32) {
-      const int mine = base + lane < rows ? (s.candidates[base + lane] + kPages - 1) / kPages : 0;
-      int sum = mine;
+      const uint32_t mine = base + lane < rows ? (s.candidates[base + lane] + kPages - 1) / kPages : 0;
+      uint32_t sum = mine;
       for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
         sum += lane >= o ? up : 0;
       }
       if (at + sum > lo && at + sum - mine <= lo) {
