@@ -258,11 +258,11 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
     ptx::tmem_alloc(ptx::smem_u32(&s.tmem), kTmemCols);
     ptx::tmem_relinquish();
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if constexpr (kWhole) row0 = blockIdx.x;
   const int request0 = row0 / p.q_len;
   const int32_t* const tables = p.block_tables + int64_t(request0) * p.block_table_stride + p.sink;  // of the first row's request, its candidates
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   Seen mine{0, 0};
   int page_of_mine = 0;  // of the candidate that this thread may take
   if constexpr (kWhole) {
