@@ -470,9 +470,10 @@ static_assert(1024 + kStages * kStageBytes + 128 * kQDim + sizeof(Small) <= 2324
 }  // namespace
 
 // Rows with at most 128 candidates have a CTA each that selects too, us in graphs, a launch each for scores and selection -> this: 16 heads, 57
-// candidates, 1 row 9.3 -> 6.9, 148 rows 11.5 -> 7.8, 296 15.9 -> 15.1; 128 heads, 127 candidates, 11.7 -> 10.1, 14.2 -> 11.0, 21.2 -> 21.6: so while
-// there are no more rows than SMs.  With two tiles, and the compares of 256 keys with one another, it was 9.6 -> 10.9.
-bool scores_and_selects(const SelectParams& p, int sms) { return p.width - p.sink - p.local <= kWholeKeys && p.batch * p.q_len <= sms; }
+// candidates, 1 row 7.9 -> 5.9, 148 rows 10.8 -> 6.7, 200 12.9 -> 12.6, 296 14.1 -> 13.1, 444 17.8 -> 19.4; 128 heads, 127 candidates, 11.0 -> 8.7,
+// 14.9 -> 9.4, 19.0 -> 17.9, 20.5 -> 18.8, 26.2 -> 28.0: so while there are no more rows than two an SM.  With two tiles, and the compares of 256
+// keys with one another, one row was 9.6 -> 10.9.
+bool scores_and_selects(const SelectParams& p, int sms) { return p.width - p.sink - p.local <= kWholeKeys && p.batch * p.q_len <= 2 * sms; }
 
 cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream) {
   const int rows = p.batch * p.q_len, columns = (p.heads + 15) / 16 * 16;
