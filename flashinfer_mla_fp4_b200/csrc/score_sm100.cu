@@ -4,9 +4,10 @@
 // largest over heads would be a reduction across threads, and fewer than 128 heads would waste half of the MMA or more.
 //
 // Bound by the gather of the pages' rows: 580 bytes a page and query position, an SM's share of the measured copy rate is a tile (128 pages,
-// 74 KB) in 1.7 us, and its 18 MMAs of 128 x 128 x 32 take 0.9.  64 requests of 2048 pages, 128 heads, up to seven tiles a CTA: 18.5 us, of which 2.1 are
-// up to the CTA's share, 3.2 the query and the first tile, 1.9 the conversion, then 1.5 a tile (7 TB/s, some of it out of L2).  So a CTA per SM
-// walks a contiguous range of the tiles of all rows, in two stages of a whole tile each: at least one tile is in flight whatever the other roles do.
+// 74 KB) in 1.7 us, and its 18 MMAs of 128 x 128 x 32 take 0.9.  64 requests of 2048 pages, 128 heads, up to seven tiles a CTA: 18 us, of which 1.8 are
+// up to the CTA's share, 3.4 the query and the first tile, 1.9 the conversion, then 1.4 a tile (8 TB/s, the queries and some rows out of L2); 21 where a
+// CTA goes on to a second row, whose query waits for the MMAs of the first.  So a CTA per SM walks a contiguous range of the tiles of all
+// rows, in two stages of a whole tile each: at least one tile is in flight whatever the other roles do.
 // Rows come by cp.async straight into the swizzled operand, 512 contiguous bytes an instruction, 32 bytes a clk and SM; a TMA gather would
 // take 160 instructions a tile.
 //
