@@ -484,7 +484,9 @@ cudaError_t launch_summarize(const SummarizeParams& p, int64_t count, int sms, c
     const auto kernel = p.page_size == 8 ? summarize_four_kernel<8> : summarize_four_kernel<16>;
     return launch_dependent(kernel, dim3(unsigned((count + 3) / 4)), kSumThreads, 0, stream, p, count);
   }
-  if (count * p.page_size >= kManyTokens && reinterpret_cast<uintptr_t>(p.kv_cache) % 32 == 0) return launch_summarize_many(p, count, sms, stream);
+  // (its tensor maps want a cache that starts on 32 bytes, its bulk copies scales that start on 16)
+  if (count * p.page_size >= kManyTokens && reinterpret_cast<uintptr_t>(p.kv_cache) % 32 == 0 && reinterpret_cast<uintptr_t>(p.kv_cache_sf) % 16 == 0)
+    return launch_summarize_many(p, count, sms, stream);
   const auto kernel = p.page_size == 32 ? summarize_kernel<32> : p.page_size == 64 ? summarize_kernel<64> : summarize_kernel<128>;
   return launch_dependent(kernel, dim3(unsigned(count)), kSumThreads, 0, stream, p);
 }

@@ -139,6 +139,13 @@ def test_summaries_of_many_pages(page):
     again, again_sf = torch.full_like(summary, 9), torch.full_like(ssf, 9.0)
     summarize_pages(odd, sf_all, again, again_sf, ids)
     assert torch.equal(again, exp) and _same(again_sf, exp_sf)
+    # ... and so do scales that start on 4
+    raw = torch.empty(sf_all.numel() + 1, device=dev)
+    odd = raw[1:].view_as(sf_all).copy_(sf_all)
+    assert odd.data_ptr() % 16 == 4
+    again.fill_(9), again_sf.fill_(9.0)
+    summarize_pages(kv_all, odd, again, again_sf, ids)
+    assert torch.equal(again, exp) and _same(again_sf, exp_sf)
 
 
 def _selection_case(lens, heads, page, q_len, seed, odd=False):
