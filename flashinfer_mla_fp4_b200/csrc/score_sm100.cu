@@ -11,7 +11,8 @@
 // Rows come by cp.async straight into the swizzled operand, 512 contiguous bytes an instruction, 32 bytes a clk and SM; a TMA gather would
 // take 160 instructions a tile.
 //
-// Few rows of one tile each (score_kernel<true>): a CTA has a row to itself, keeps its keys in shared memory and selects too, by counting for each page
+// Several query positions of a request look at the same pages: where their heads fit into 128 columns side by side, and there are tiles enough, one load of
+// a tile serves them all (Form::kTogether).  Few rows of one tile each (Form::kWhole): a CTA has a row to itself, keeps its keys in shared memory and selects too, by counting for each page
 // those before it: no second launch, and nothing that another CTA has to see.
 //
 // Roles: warps 0-3 take the scores out of TMEM, warp 4 issues the MMAs, warps 5-20 load, and turn a row's query into integers (the B
@@ -130,14 +131,21 @@ __device__ __forceinline__ void copy_rows(uint32_t operand, int rows, int first,
   }
 }
 
+// columns of the MMAs for the heads of a query position
+__host__ __device__ __forceinline__ int columns_of(int heads) { return (heads + 15) / 16 * 16; }
+
 // The heads of a row's query, to be the B operand: first fetched as they are, ...  Columns behind the last head repeat head 0, which leaves the
-// largest score as it is.
+// largest score as it is.  kTogether: of all query positions of the request, `row` being the first.
+template <bool kTogether>
 __device__ __forceinline__ void fetch_b(const SelectParams& p, uint32_t b_smem, int row, int columns) {
   const int each = columns / kLoadWarps, first = ((threadIdx.x >> 5) - kFirstLoad) * each, batch = row / p.q_len;
   const uint8_t* q = p.q + batch * p.q_stride_batch + (row - batch * p.q_len) * p.q_stride_qpos;
+  // 2^16 / the columns of a position, and up to one more: a product with a column is off by less than 2^-8, and a quotient that is not whole has at least 2^-6
+  // to the next one
+  const int inverse = kTogether ? int(65536.f * __frcp_rn(float(columns_of(p.heads)))) + 1 : 0;
   copy_rows(b_smem, columns, first, each, [&](int r) {
-    const int head = first + r;
-    return reinterpret_cast<const char*>(q + (head < p.heads ? head : 0) * p.q_stride_head);
+    const int position = kTogether ? (first + r) * inverse >> 16 : 0, head = first + r - position * columns_of(p.heads);
+    return reinterpret_cast<const char*>(q + (kTogether ? position * p.q_stride_qpos : 0) + (head < p.heads ? head : 0) * p.q_stride_head);
   });
 }
 // ... then turned into integers where they lie: eight lanes a head, four heads at a time.  In FP16: an E4M3 value times 2^k is exact, and adding 1536
@@ -232,9 +240,13 @@ __device__ __forceinline__ void select_whole(const SelectParams& p, Small& s, in
   out[at] = page;
 }
 
-// kWhole: CTA i has row i and selects; else the CTAs share the tiles of rows row0 to row0 + rows - 1.
-template <bool kWhole>
+// kWhole: CTA i has row i and selects; else the CTAs share the tiles of rows row0 to row0 + rows - 1; kTogether: of requests, all of whose query positions
+// are scored with one load of a tile.
+enum class Form { kRows, kWhole, kTogether };
+template <Form kForm>
 __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int row0, int rows, int columns) {
+  constexpr bool kWhole = kForm == Form::kWhole, kTogether = kForm == Form::kTogether;
+  const int positions = kTogether ? p.q_len : 1;  // of a row here
   extern __shared__ char raw[];
   char* a_smem = raw + ((1024 - (ptx::smem_u32(raw) & 1023)) & 1023);
   char* b_smem = a_smem + kStages * kStageBytes;
@@ -260,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
     ptx::tmem_relinquish();
   }
   if constexpr (kWhole) row0 = blockIdx.x;
-  const int request0 = row0 / p.q_len;
+  const int request0 = kTogether ? row0 : row0 / p.q_len;
   const int32_t* const tables = p.block_tables + int64_t(request0) * p.block_table_stride + p.sink;  // of the first row's request, its candidates
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -281,8 +293,8 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
     }
   } else {
     for (int r = tid; r < rows; r += kThreads) {
-      const Seen v = seen(p, row0 + r);
-      s.request[r] = uint16_t((row0 + r) / p.q_len - request0);
+      const Seen v = seen(p, kTogether ? (row0 + r) * positions + positions - 1 : row0 + r);  // (the last position sees the most)
+      s.request[r] = uint16_t(kTogether ? r : (row0 + r) / p.q_len - request0);
       s.candidates[r] = v.used > p.budget ? v.used - p.sink - p.local : 0;
     }
   }
@@ -324,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
       // A row's query is fetched once the MMAs of the row before are over, which is known where the tile behind its first one is loaded; the
       // first row's before anything, and converted while the first tile is on its way (behind the second one: 24.4 us instead of 23.6 for 32 rows of
       // 2048 pages).
-      fetch_b(p, b_addr, row0 + k.row, columns);
+      fetch_b<kTogether>(p, b_addr, (row0 + k.row) * positions, columns);
       asm volatile("cp.async.commit_group;" ::: "memory");
       // Page numbers are asked for two tiles ahead, and before the rows: behind those they would take as long.
       Walk ahead(s);
@@ -339,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         if (n >= kStages && (more || fresh >= 0)) ok = wait(c, s.empty_a[st], ((n >> 1) - 1) & 1);
         if (!ok) break;
         if (fresh >= 0) {
-          fetch_b(p, b_addr, row0 + fresh, columns);
+          fetch_b<kTogether>(p, b_addr, (row0 + fresh) * positions, columns);
           asm volatile("cp.async.commit_group;" ::: "memory");
         }
         const int next_fresh = more && n > 0 && k.tile == 0 ? k.row : -1;
@@ -435,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
         const float* unit = s.unit[seg & 3];
         ptx::tc_fence_after();
         float best = __uint_as_float(0xff800000u);
+        int position = 0, end = columns_of(p.heads);
 #pragma unroll 1
         for (int col = 0; col < columns; col += 16) {
           uint32_t d[16];
@@ -445,13 +458,23 @@ __global__ void __launch_bounds__(kThreads, 1) score_kernel(SelectParams p, int 
           ptx::tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 16; ++j) best = fmaxf(best, float(int(d[j])) * u[j]);
+          if constexpr (kTogether) {
+            if (col + 16 < end) continue;
+            // (a position that sees fewer pages than the last one has room for the keys all the same, and nobody reads them)
+            if (scored) p.keys[(int64_t(row0 + row) * positions + position) * p.key_stride + i] = there ? key_of(best * scale) : 0u;
+            ++position;
+            end += columns_of(p.heads);
+            best = __uint_as_float(0xff800000u);
+          }
         }
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(s.empty_d[st]));
-        const uint32_t key = there ? key_of(best * scale) : 0u;
-        if (kWhole && scored) s.keys[i] = key;
-        if (!kWhole && scored) p.keys[int64_t(row0 + row) * p.key_stride + i] = key;
+        if constexpr (!kTogether) {
+          const uint32_t key = there ? key_of(best * scale) : 0u;
+          if (kWhole && scored) s.keys[i] = key;
+          if (!kWhole && scored) p.keys[int64_t(row0 + row) * p.key_stride + i] = key;
+        }
         seg += last;
       }
     }
@@ -477,18 +500,26 @@ static_assert(1024 + kStages * kStageBytes + 128 * kQDim + sizeof(Small) <= 2324
 bool scores_and_selects(const SelectParams& p, int sms) { return p.width - p.sink - p.local <= kWholeKeys && p.batch * p.q_len <= 2 * sms; }
 
 cudaError_t launch_score(const SelectParams& p, int sms, cudaStream_t stream) {
-  const int rows = p.batch * p.q_len, columns = (p.heads + 15) / 16 * 16;
-  const size_t smem = smem_bytes(columns);
-  static std::atomic<bool> allowed[2][64];
-  cudaError_t e = allow_smem(score_kernel<false>, smem_bytes(128), allowed[0]);
-  if (e == cudaSuccess) e = allow_smem(score_kernel<true>, smem_bytes(128), allowed[1]);
+  const int rows = p.batch * p.q_len, columns = columns_of(p.heads);
+  static std::atomic<bool> allowed[3][64];
+  cudaError_t e = allow_smem(score_kernel<Form::kRows>, smem_bytes(128), allowed[0]);
+  if (e == cudaSuccess) e = allow_smem(score_kernel<Form::kWhole>, smem_bytes(128), allowed[1]);
+  if (e == cudaSuccess) e = allow_smem(score_kernel<Form::kTogether>, smem_bytes(128), allowed[2]);
   if (e != cudaSuccess) return e;
-  if (scores_and_selects(p, sms)) return launch_dependent(score_kernel<true>, dim3(unsigned(rows)), kThreads, smem, stream, p, 0, 1, columns);
+  if (scores_and_selects(p, sms))
+    return launch_dependent(score_kernel<Form::kWhole>, dim3(unsigned(rows)), kThreads, smem_bytes(columns), stream, p, 0, 1, columns);
   const int64_t tiles = (p.width - p.sink - p.local + kPages - 1) / kPages;  // of the longest row that the tables can hold
-  for (int row0 = 0; row0 < rows; row0 += kMaxRows) {
-    const int n = rows - row0 < kMaxRows ? rows - row0 : kMaxRows;
+  // Query positions of a request together, where their heads fit side by side, us in graphs, a row each -> together, 16 heads: three positions of 32
+  // requests of 2048 pages (1536 tiles of rows) 24.5 -> 17.0, of 8 (384) 13.6 -> 10.8, of 8 of 512 pages (96) 8.5 -> 9.1; two of 8 of 2048 (256) 10.7 -> 10.2;
+  // eight of 16 of 512 (512) 14.3 -> 12.1, of 8 of 512 (256) 11.0 -> 11.2; 64 heads, two positions of 32 of 2048 21.6 -> 20.8, of 8 (256) 11.5 -> 12.4: so
+  // where the rows have more than two tiles an SM (few tiles leave SMs idle, and each converts all positions' queries).
+  const bool together = p.q_len > 1 && p.q_len * columns <= 128 && tiles * rows > 2 * sms;
+  const auto kernel = together ? score_kernel<Form::kTogether> : score_kernel<Form::kRows>;
+  const int all = together ? p.batch : rows, wide = together ? p.q_len * columns : columns;
+  for (int row0 = 0; row0 < all; row0 += kMaxRows) {
+    const int n = all - row0 < kMaxRows ? all - row0 : kMaxRows;
     const int64_t most = tiles * n;
-    e = launch_dependent(score_kernel<false>, dim3(unsigned(most < sms ? most : sms)), kThreads, smem, stream, p, row0, n, columns);
+    e = launch_dependent(kernel, dim3(unsigned(most < sms ? most : sms)), kThreads, smem_bytes(wide), stream, p, row0, n, wide);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

@@ -190,7 +190,12 @@ def _selection_case(lens, heads, page, q_len, seed, odd=False):
     ([140000, 131200], 8, 8, 1, 700, 1, 2, False, True),  # more candidates than a CTA's registers hold
     ([1030] * 1100, 4, 128, 1, 8, 1, 2, False, False),  # more rows than a launch, hardly a tile each
     ([300, 9000, 17, 1100, 0, 128 * 130], 112, 8, 2, 20, 1, 2, True, True),  # tiles of different rows in turn
-    ([700, 1500, 90] * 134, 4, 8, 3, 8, 1, 2, True, True),  # a launch that ends inside a request
+    ([300, 90] * 200, 70, 8, 3, 8, 1, 2, True, True),  # a launch that ends inside a request
+    ([131000, 2401, 2400, 2402, 0], 8, 8, 3, 300, 1, 2, True, True),  # positions together; some of a request within the budget, others not
+    ([70000, 0, 69999, 8 * 40 + 1], 20, 16, 4, 16, 0, 1, True, True),
+    ([70000, 0, 69999, 8 * 40 + 1], 64, 16, 2, 16, 1, 2, False, True),
+    ([700, 1500, 90] * 134, 4, 8, 3, 8, 1, 2, True, True),
+    ([300, 90] * 550, 3, 8, 2, 8, 1, 2, True, False),  # ... of more requests than a launch
     ([1030, 50, 900] * 30, 6, 8, 3, 8, 1, 2, True, True),  # a CTA a row, more of them than SMs
 ])
 def test_selection_equals_the_oracle(lens, heads, page, q_len, budget, sink, local, causal, odd):
