@@ -11,14 +11,14 @@
 // Rows come by cp.async straight into the swizzled operand, 512 contiguous bytes an instruction, 32 bytes a clk and SM; a TMA gather would
 // take 160 instructions a tile.
 //
-// Several query positions of a request look at the same pages: where their heads fit into 128 columns side by side, and there are tiles enough, one load of
-// a tile serves them all (Form::kTogether).  Few rows of one tile each (Form::kWhole): a CTA has a row to itself, keeps its keys in shared memory and selects too, by counting for each page
-// those before it: no second launch, and nothing that another CTA has to see.
+// Several query positions of a request look at the same pages: where their heads fit into 128 columns side by side, and there are tiles enough,
+// one load of a tile serves them all (Form::kTogether).  Few rows of one tile each (Form::kWhole): a CTA has a row to itself, keeps its keys in
+// shared memory and selects too, by counting for each page those before it: no second launch, and nothing that another CTA has to see.
 //
 // Roles: warps 0-3 take the scores out of TMEM, warp 4 issues the MMAs, warps 5-20 load, and turn a row's query into integers (the B
-// operand) while the row's first tile is on its way.  (With eight warps for that instead of sixteen 32 requests of 2048 pages, 128 heads, with their
-// attention took 67.7 us instead of 66.0, 64 such selections 28.1 instead of 27.2; one of 16 heads 7.6 instead of 8.0.)  All waits are bounded; one that runs out sets the status and ends the CTA, whose
-// keys are then not all written.
+// operand) while the row's first tile is on its way.  (With eight warps for that instead of sixteen 32 requests of 2048 pages, 128 heads, with
+// their attention took 67.7 us instead of 66.0, 64 such selections 28.1 instead of 27.2; one of 16 heads 7.6 instead of 8.0.)  All waits are
+// bounded; one that runs out sets the status and ends the CTA, whose keys are then not all written.
 #include "common.cuh"
 #include "launch.h"
 #include "ptx_sm100.cuh"
