@@ -81,12 +81,13 @@ class FP4MLAPagePool:
     def __init__(self, caches: Sequence[FP4MLAPagedCache]) -> None:
         self.caches = list(caches)
         self._array, self.num_pages, self.page_size, self.device, self._kept = _layers(self.caches)
+        self._address = C.addressof(self._array)
         self.refcounts = torch.zeros(self.num_pages, dtype=torch.int32, device=self.device)
         self._status = torch.zeros(8, dtype=torch.int32, device=self.device)
 
     def _native(self, what: int, block_tables, seq_lens, x, y=None):
         """The common form of a call, checked and launched natively; None: nothing was done."""
-        return _cabi.native.pool(what, C.addressof(self._array), len(self._array), self.page_size, self.num_pages, self.refcounts, self._status,
+        return _cabi.native.pool(what, self._address, len(self._array), self.page_size, self.num_pages, self.refcounts, self._status,
                                   block_tables, seq_lens, x, y)
 
     def num_free(self) -> int:

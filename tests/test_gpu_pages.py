@@ -155,6 +155,24 @@ def test_random_histories(seed, page, layers, pages, rows, width):
         _check(pool, caches, before, want, bt, sl)
 
 
+@pytest.mark.parametrize("pages", [1, 8, 9, 8191, 8192, 8193])
+@pytest.mark.parametrize("use", ["all", "none", "the first", "the last", "all but the first"])
+def test_compaction_at_the_ends(pages, use):
+    """Pools of about what a planning CTA looks at in a round, with a list of new numbers that starts anywhere."""
+    from flashinfer_mla_fp4_b200 import FP4MLAPagePool
+
+    caches = _caches(1, pages, 8, False)
+    pool = FP4MLAPagePool(caches)
+    used = {"all": range(pages), "none": (), "the first": (0,), "the last": (pages - 1,), "all but the first": range(1, pages)}[use]
+    pool.refcounts[list(used)] = 3
+    bt, sl = torch.zeros(1, 2, dtype=torch.int32, device=_dev()), _i32([0])
+    want, before = S.Pool(pool.refcounts.tolist(), bt.tolist(), sl.tolist(), 8), _bytes(caches)
+    remap = torch.full((pages + 2,), -9, dtype=torch.int32, device=_dev())
+    assert pool.compact(bt, sl, remap[1:-1]).tolist() == want.compact()
+    assert int(remap[0]) == -9 and int(remap[-1]) == -9
+    _check(pool, caches, before, want, bt, sl)
+
+
 def test_a_pool_that_runs_out():
     from flashinfer_mla_fp4_b200 import FP4MLAPagePool
 
