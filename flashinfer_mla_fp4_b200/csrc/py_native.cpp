@@ -21,6 +21,8 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/CachingHostAllocator.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
@@ -380,6 +382,11 @@ bool query_ok(const at::Tensor& q) {
   return q.is_cuda() && q.dim() == 4 && q.scalar_type() == at::kFloat8_e4m3fn && q.size(3) == MLA_FP4_LATENT_DIM + MLA_FP4_ROPE_DIM && q.stride(3) == 1 &&
          q.size(0) > 0 && q.size(1) > 0 && q.size(2) > 0 && q.size(2) <= 128;
 }
+// A tensor on the current device for results that a kernel writes in full, and memory for a call's own use: at::empty without its dispatch, of which
+// three in a call were a fifth of its time on the host.
+at::Tensor room(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) { return at::Tensor(at::detail::empty_cuda(shape, type, dev, std::nullopt)); }
+c10::DataPtr scratch(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
+
 // summarize(kv_cache, kv_cache_sf, summary, summary_sf, page_ids, block_tables, seq_lens, new_tokens, status or None) -> whether it was launched; page_ids, or
 // the other three
 PyObject* summarize(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -483,14 +490,14 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int rc;
   {
     NoGil released;
-    const auto ints = at::TensorOptions().dtype(at::kInt).device(dev);
-    if (!out[0].defined()) out[0] = at::empty({rows, b.budget}, ints);
-    if (!out[1].defined()) out[1] = at::empty({rows}, ints);
-    if (!out[2].defined()) out[2] = at::empty({int64_t(need)}, at::TensorOptions().dtype(at::kChar).device(dev));
+    if (!out[0].defined()) out[0] = room({rows, b.budget}, at::kInt, dev);
+    if (!out[1].defined()) out[1] = room({rows}, at::kInt, dev);
     s.selected = static_cast<int32_t*>(out[0].data_ptr());
     s.selected_lens = static_cast<int32_t*>(out[1].data_ptr());
-    s.workspace = out[2].data_ptr();
-    s.workspace_bytes = size_t(out[2].numel());
+    c10::DataPtr own;
+    if (!out[2].defined() && need > 0) own = scratch(need);
+    s.workspace = out[2].defined() ? out[2].data_ptr() : own.get();
+    s.workspace_bytes = out[2].defined() ? size_t(out[2].numel()) : need;
     rc = abi.select_pages(&s);
   }
   if (rc != MLA_FP4_OK) return raise_status(rc);
@@ -593,8 +600,8 @@ PyObject* sparse_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int rc;
   {
     NoGil released;
-    if (!given) out = at::empty(at::IntArrayRef(shape, 4), at::TensorOptions().dtype(out_type).device(dev));
-    if (want_lse && !lse_given) lse = at::empty(at::IntArrayRef(shape, 3), at::TensorOptions().dtype(at::kFloat).device(dev));
+    if (!given) out = room(at::IntArrayRef(shape, 4), out_type, dev);
+    if (want_lse && !lse_given) lse = room(at::IntArrayRef(shape, 3), at::kFloat, dev);
     d.out = out.data_ptr();
     d.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
     rc = abi.select_pages(&s);
@@ -655,13 +662,13 @@ PyObject* pool(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int rc;
   {
     NoGil released;
-    at::Tensor workspace = at::empty({int64_t(need)}, at::TensorOptions().dtype(at::kChar).device(dev));
-    p.workspace = workspace.data_ptr();
+    const c10::DataPtr own = scratch(need);
+    p.workspace = own.get();
     if (what == 0) rc = abi.pool_allocate(&p, xp);
     else if (what == 1) rc = abi.pool_fork(&p, xp, yp, int32_t(count));
     else if (what == 2) rc = abi.pool_free(&p, xp, int32_t(count));
     else {
-      remap = x ? *x : at::empty({pages}, at::TensorOptions().dtype(at::kInt).device(dev));
+      remap = x ? *x : room({pages}, at::kInt, dev);
       rc = abi.pool_compact(&p, static_cast<int32_t*>(remap.data_ptr()));
     }
   }
