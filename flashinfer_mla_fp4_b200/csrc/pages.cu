@@ -150,17 +150,34 @@ __global__ void __launch_bounds__(kPlanThreads, 1) allocate_kernel(PoolParams p,
   }
   const int found = for_free_pages(p.refcounts, p.num_pages, int(min(total, (long long)(p.num_pages))), warp_s, counts, [&](int number, int page) { list[number] = page; });
   __syncthreads();
-  for (int r = threadIdx.x >> 5; r < p.rows; r += kPlanThreads / 32) {
-    const int have = pages_of(p.seq_lens[r], p.page_size), want = pages_of(new_lens[r], p.page_size), at = offset[r];
-    if (want > p.width || want <= have) continue;
-    if (at + want - have > found) {
-      if ((threadIdx.x & 31) == 0) report(p.status, kPoolOutOfPages, r);
-      continue;
+  // A thread writes up to four pages of its row, a warp longer rows in turn (a warp per row: 1024 rows with two new pages each 20.4 us,
+  // 64 rows 4.3; so 5.5 and 3.5).
+  constexpr int kFewPages = 4;
+  const int lane = threadIdx.x & 31;
+  const auto give = [&](int r, int have, int at, int k) {
+    const int page = list[at + k];
+    p.block_tables[int64_t(r) * p.block_table_stride + have + k] = page;
+    p.refcounts[page] = 1;
+  };
+  for (int base = 0; base < p.rows; base += kPlanThreads) {
+    const int r = base + threadIdx.x;
+    int have = 0, need = 0, at = 0;
+    if (r < p.rows) {
+      have = pages_of(p.seq_lens[r], p.page_size);
+      const int want = pages_of(new_lens[r], p.page_size);
+      at = offset[r];
+      if (want <= p.width && want > have) need = want - have;
+      if (need > 0 && int64_t(at) + need > found) {
+        report(p.status, kPoolOutOfPages, r);
+        need = 0;
+      }
     }
-    for (int k = threadIdx.x & 31; k < want - have; k += 32) {
-      const int page = list[at + k];
-      p.block_tables[int64_t(r) * p.block_table_stride + have + k] = page;
-      p.refcounts[page] = 1;
+    if (need <= kFewPages)
+      for (int k = 0; k < need; ++k) give(r, have, at, k);
+    for (uint32_t more = __ballot_sync(0xffffffffu, need > kFewPages); more; more &= more - 1) {
+      const int of = __ffs(more) - 1, row = r - lane + of, held = __shfl_sync(0xffffffffu, have, of), start = __shfl_sync(0xffffffffu, at, of),
+                pages = __shfl_sync(0xffffffffu, need, of);
+      for (int k = lane; k < pages; k += 32) give(row, held, start, k);
     }
   }
 }
