@@ -433,6 +433,7 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
           if (before == rest && lane == 0) least_s = place;
         }
       } else {  // all of one key: the first ones
+        __syncthreads();  // (where no round was needed, a warp may still be reading the keys' range, whose place the scan takes)
         uint32_t equal = 0;
         for_keys([&](uint32_t key, int, int) { equal += key == low; });
         uint32_t before = scan(equal) - equal;
