@@ -58,14 +58,20 @@ struct Ctx {
   const SelectParams& p;
   Small& s;
 };
-// Bounded: false when it ran out, here or in another role.
+// Of a whole warp, and bounded: false when it ran out, here or in another role.  The answer is the same in all lanes: one that gave up alone would leave
+// the others in front of what a warp does together.
 __device__ __forceinline__ bool wait(const Ctx& c, const unsigned long long& b, uint32_t parity) {
-  for (uint32_t i = 0; i < c.p.wait_polls; ++i) {
-    if (ptx::mbar_try_wait(bar(b), parity)) return true;
-    if (c.s.abort) return false;
+  bool there = false;
+  for (uint32_t i = 0; i < c.p.wait_polls && !c.s.abort; ++i) {
+    there = ptx::mbar_try_wait(bar(b), parity);
+    if (there) break;
   }
-  c.s.abort = 1;
-  report_timeout(c.p.status, bar(b), parity);
+  if (__all_sync(0xffffffffu, there)) return true;
+  if ((threadIdx.x & 31) == 0 && !c.s.abort) {
+    c.s.abort = 1;
+    report_timeout(c.p.status, bar(b), parity);
+  }
+  __syncwarp();
   return false;
 }
 
