@@ -114,14 +114,13 @@ __device__ __forceinline__ int summary_code(int sum, float scale, float by, floa
   return scale > 0.f ? int(fminf(fmaxf(whole, -127.f), 127.f)) : 0;
 }
 
-// what a bounded wait that ran out leaves in the status words
+// what a bounded wait that ran out leaves in the status words: the first one's record, as in the decode kernel
 __device__ __forceinline__ void report_timeout(int32_t* status, uint32_t bar, uint32_t parity) {
-  if (!status) return;
+  if (!status || atomicCAS(status, 0, MLA_FP4_ERR_DEVICE_TIMEOUT) != 0) return;
   status[1] = int(bar);
   status[2] = blockIdx.x;
   status[3] = threadIdx.x;
   status[4] = int(parity);
-  status[0] = MLA_FP4_ERR_DEVICE_TIMEOUT;
 }
 
 }  // namespace mla

@@ -41,39 +41,54 @@ def test_rows_of_pages_that_all_tie(pages, rows, of):
         assert bool((lens == budget * 8 - 3).all())
 
 
-def test_a_wait_that_runs_out_for_certain():
-    """A poll budget of one where a CTA waits for longer than a poll may take: 1984 tiles, 128 heads, inputs that are not in L2.  The status says so, the kernel
-    ends, what is selected are pages of the request, and the next call is right."""
-    dev = _dev()
-    from flashinfer_mla_fp4_b200 import _cabi
-    from flashinfer_mla_fp4_b200.sparse import select_pages
+class _Slow:
+    """A selection of 124 rows of 2048 pages, 128 heads, from inputs that are not in L2: with a poll budget of one a wait runs out for certain."""
 
-    rows, pages, budget = 124, 2048, 64
-    q, summary, ssf, bt, sl = (t.to(dev) for t in _selection_case([pages * 64] * rows, 128, 64, 1, seed=4))
-    want, want_lens = select_pages(q, summary, ssf, bt, sl, 64, budget)
-    sel, lens = torch.empty_like(want), torch.empty_like(want_lens)
-    ws, status = torch.zeros(_cabi.select_workspace_bytes(rows, 1, pages), dtype=torch.int8, device=dev), torch.zeros(8, dtype=torch.int32, device=dev)
-    a = _cabi.SelectArgs()
-    a.q, a.q_stride_batch, a.q_stride_qpos, a.q_stride_head = q.data_ptr(), q.stride(0), q.stride(1), q.stride(2)
-    a.summary, a.summary_sf, a.num_pages = summary.data_ptr(), ssf.data_ptr(), summary.shape[0]
-    a.block_tables, a.block_table_stride, a.seq_lens = bt.data_ptr(), bt.stride(0), sl.data_ptr()
-    a.selected, a.selected_lens, a.workspace, a.workspace_bytes = sel.data_ptr(), lens.data_ptr(), ws.data_ptr(), ws.numel()
-    a.batch, a.q_len, a.num_heads, a.page_size, a.width = rows, 1, 128, 64, pages
-    a.budget, a.sink_pages, a.local_pages, a.status = budget, 1, 2, status.data_ptr()
-    a.stream = torch.cuda.current_stream().cuda_stream
-    cold = torch.empty(300 << 20, dtype=torch.uint8, device=dev)
-    for i in range(3):
-        a.wait_polls = 1
-        status.zero_()
-        cold.fill_(i)
-        _cabi.check(_cabi.lib.mla_fp4_select_pages(C.byref(a)))
+    def __init__(self):
+        from flashinfer_mla_fp4_b200 import _cabi
+        from flashinfer_mla_fp4_b200.sparse import select_pages
+
+        dev, rows, pages, budget = _dev(), 124, 2048, 64
+        self.inputs = q, summary, ssf, bt, sl = [t.to(dev) for t in _selection_case([pages * 64] * rows, 128, 64, 1, seed=4)]
+        self.bt, self.want = bt, select_pages(q, summary, ssf, bt, sl, 64, budget)
+        self.sel, self.lens = (torch.empty_like(t) for t in self.want)
+        self.ws = torch.zeros(_cabi.select_workspace_bytes(rows, 1, pages), dtype=torch.int8, device=dev)
+        self.status, self.cold = torch.zeros(8, dtype=torch.int32, device=dev), torch.empty(300 << 20, dtype=torch.uint8, device=dev)
+        a = self.args = _cabi.SelectArgs()
+        a.q, a.q_stride_batch, a.q_stride_qpos, a.q_stride_head = q.data_ptr(), q.stride(0), q.stride(1), q.stride(2)
+        a.summary, a.summary_sf, a.num_pages = summary.data_ptr(), ssf.data_ptr(), summary.shape[0]
+        a.block_tables, a.block_table_stride, a.seq_lens = bt.data_ptr(), bt.stride(0), sl.data_ptr()
+        a.selected, a.selected_lens, a.workspace, a.workspace_bytes = self.sel.data_ptr(), self.lens.data_ptr(), self.ws.data_ptr(), self.ws.numel()
+        a.batch, a.q_len, a.num_heads, a.page_size, a.width = rows, 1, 128, 64, pages
+        a.budget, a.sink_pages, a.local_pages, a.status = budget, 1, 2, self.status.data_ptr()
+        a.stream = torch.cuda.current_stream().cuda_stream
+
+    def run(self, polls, status=(0,) * 8):
+        """The status words after a call with that poll budget."""
+        from flashinfer_mla_fp4_b200 import _cabi
+
+        self.status.copy_(torch.tensor(status, dtype=torch.int32))
+        self.cold.fill_(polls)
+        self.args.wait_polls = polls
+        _cabi.check(_cabi.lib.mla_fp4_select_pages(C.byref(self.args)))
         torch.cuda.synchronize()
-        code, _, cta, thread, parity = status[:5].tolist()
+        return self.status.tolist()
+
+
+def test_a_wait_that_runs_out_for_certain():
+    """The status says so, the kernel ends, what is selected are pages of the request, and the next call is right."""
+    slow = _Slow()
+    from flashinfer_mla_fp4_b200 import _cabi
+
+    for _ in range(3):
+        code, _, cta, thread, parity = slow.run(1)[:5]
         assert code == _cabi.ERR_DEVICE_TIMEOUT and 0 <= cta < 148 and thread % 32 == 0 and parity in (0, 1)  # one warp's record
-        assert torch.equal(lens, want_lens)
-        assert bool((sel.unsqueeze(2) == bt.unsqueeze(1)).any(2).all())
-        a.wait_polls = 0
-        status.zero_()
-        _cabi.check(_cabi.lib.mla_fp4_select_pages(C.byref(a)))
-        torch.cuda.synchronize()
-        assert int(status[0]) == 0 and torch.equal(sel, want) and torch.equal(lens, want_lens)
+        assert torch.equal(slow.lens, slow.want[1])
+        assert bool((slow.sel.unsqueeze(2) == slow.bt.unsqueeze(1)).any(2).all())
+        assert slow.run(0)[0] == 0 and torch.equal(slow.sel, slow.want[0]) and torch.equal(slow.lens, slow.want[1])
+
+
+def test_the_first_record_of_a_wait_that_ran_out_stays():
+    """A status that nobody has looked at yet keeps what it says, as with the decode kernel, whose status words sparse decode shares."""
+    slow, before = _Slow(), [5, 1, 2, 3, 4, 9, 9, 9]
+    assert slow.run(1, before) == before
