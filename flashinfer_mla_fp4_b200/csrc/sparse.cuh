@@ -101,7 +101,8 @@ __device__ __forceinline__ float summary_scale(int most_lat, int most_rope, floa
 }
 // round(sum * top * unit / scale), within [-127, 127]; 0 where the scale is 0 or NaN.  `by` is top * unit / scale in FP32, and will do unless the
 // product is too near the middle of two whole numbers (it is off by less than 2^-14: roundings of 5 * 127 half-ulps of 1): then the
-// sum is compared with the middle in 64 bits.
+// sum is compared with the middle in 64 bits.  A sum of 0 is code 0 whatever `by` is: beside a part of the page that outweighs it beyond FP32, `by` may be
+// infinite, which no other sum can meet (the scale is at least |sum| * top * unit / 127, and half that where it is subnormal).
 __device__ __forceinline__ int summary_code(int sum, float scale, float by, float top, double unit) {
   const float x = float(sum) * by;
   float whole = rintf(x);
@@ -111,7 +112,7 @@ __device__ __forceinline__ int summary_code(int sum, float scale, float by, floa
     const float toward = copysignf(0.5f, x);
     whole = over == 0.0 ? rintf(middle) : (over > 0.0) == (x > 0.f) ? middle + toward : middle - toward;
   }
-  return scale > 0.f ? int(fminf(fmaxf(whole, -127.f), 127.f)) : 0;
+  return scale > 0.f && sum != 0 ? int(fminf(fmaxf(whole, -127.f), 127.f)) : 0;
 }
 
 // what a bounded wait that ran out leaves in the status words: the first one's record, as in the decode kernel

@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from test_gpu_sparse import E4M3, _dev, _selection_case
+from test_gpu_sparse import E4M3, _dev, _oracle_summaries, _pages, _same, _selection_case
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,37 @@ def test_the_first_record_of_a_wait_that_ran_out_stays():
     """A status that nobody has looked at yet keeps what it says, as with the decode kernel, whose status words sparse decode shares."""
     slow, before = _Slow(), [5, 1, 2, 3, 4, 9, 9, 9]
     assert slow.run(1, before) == before
+
+
+def _one_sided_pages(page):
+    """Pages one part of whose summary is nothing beside the other: the factor that takes a sum to a code is beyond FP32 where the sums are all zero."""
+    kv, sf = _pages(12, page, page + 7)
+    kv[:6, :, :256] = 0
+    kv[:6, :, 256:] = 0x30  # RoPE 0.5 throughout, latent zero under huge scales
+    for i, scale in enumerate((1e30, 1e37, 3e38, -3e38)):
+        sf[i] = scale
+    kv[4, 0, 3], sf[4] = 0x21, 1e37  # ... one latent value that is not
+    sf[5] = 0.0
+    kv[6:, :, 256:] = 0  # RoPE zero, scales whose means are subnormal
+    for i, scale in enumerate((1e-41, 3e-42, 1e-39, -1e-41)):
+        sf[6 + i] = scale
+    kv[6:10, 0, :256] = 0x77  # (a mean that does not round to zero)
+    kv[10, :, 256], kv[10, :, 257], sf[10] = 0x01, 0x81, 1e-41  # RoPE values of 2^-9: beside them the latent is nothing
+    return kv, sf
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128])
+def test_summaries_of_pages_with_one_empty_part(page):
+    dev = _dev()
+    from flashinfer_mla_fp4_b200.sparse import summarize_pages
+
+    kv, sf = _one_sided_pages(page)
+    want, want_sf = _oracle_summaries(kv, sf)
+    assert not want[:4, :512].any() and not want[6:10, 512:].any() and bool((want_sf[6:10] > 0).all())
+    for copies in (1, 140000 // (12 * page) + 1):  # a few pages, and enough for the tensor cores
+        kvd, sfd, n = kv.repeat(copies, 1, 1).to(dev), sf.repeat(copies, 1, 1).to(dev), 12 * copies
+        summary, ssf = torch.full((n, 576), 9, dtype=torch.int8, device=dev), torch.full((n,), 9.0, device=dev)
+        summarize_pages(kvd, sfd, summary, ssf, torch.arange(n, dtype=torch.int32, device=dev))
+        for i in range(12):
+            assert torch.equal(summary.view(copies, 12, 576)[:, i].cpu(), want[i].expand(copies, -1)), (copies, i)
+        assert _same(ssf.cpu(), want_sf.repeat(copies))
