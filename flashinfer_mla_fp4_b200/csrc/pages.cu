@@ -135,23 +135,53 @@ __global__ void __launch_bounds__(kPlanThreads, 1) allocate_kernel(PoolParams p,
   dependent_launch();
   const Counts counts(p.refcounts, 0, p.num_pages);
   int32_t *offset = p.ws, *list = p.ws + p.rows;
+  const auto demand = [&](int r) {  // new pages of a row that has room for them in its table, else none
+    const int have = pages_of(p.seq_lens[r], p.page_size), want = pages_of(new_lens[r], p.page_size);
+    return want <= p.width && want > have ? want - have : 0;
+  };
   long long total = 0;  // (rows may ask for more than 32 bits hold)
   for (int base = 0; base < p.rows; base += kPlanThreads) {
     const int r = base + threadIdx.x;
     long long need = 0, sum;
     if (r < p.rows) {
-      const int have = pages_of(p.seq_lens[r], p.page_size), want = pages_of(new_lens[r], p.page_size);
-      if (want > p.width) report(p.status, kPoolBadRow, r);
-      else if (want > have) need = want - have;
+      if (pages_of(new_lens[r], p.page_size) > p.width) report(p.status, kPoolBadRow, r);
+      need = demand(r);
     }
     const long long at = total + scan_before(need, sum_s, &sum);
     if (r < p.rows) offset[r] = int(min(at, (long long)(p.num_pages)));
     total += sum;
   }
   const int found = for_free_pages(p.refcounts, p.num_pages, int(min(total, (long long)(p.num_pages))), warp_s, counts, [&](int number, int page) { list[number] = page; });
+  // Not enough for all: a row that does not fit (offset -1) leaves what there is to those behind it.  One warp goes over the rows in order, 32 at a time: those
+  // up to the first that does not fit are served, then the same again with those behind it that still may.
+  if (total > found && threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int next = 0;
+    for (int base = 0; base < p.rows; base += 32) {
+      const int r = base + lane, need = r < p.rows ? demand(r) : 0;
+      int at = -1;
+      for (uint32_t open = __ballot_sync(0xffffffffu, need > 0); open;) {
+        const int left = found - next;
+        open = __ballot_sync(0xffffffffu, (open >> lane & 1) && need <= left);
+        const long long mine = open >> lane & 1 ? need : 0;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long up = __shfl_up_sync(0xffffffffu, upto, o);
+          upto += lane >= o ? up : 0;
+        }
+        const uint32_t over = __ballot_sync(0xffffffffu, mine > 0 && upto > left);
+        const int first = over ? __ffs(over) - 1 : 32;
+        if (mine > 0 && lane < first) at = next + int(upto - mine);
+        next += int(__shfl_sync(0xffffffffu, over ? upto - mine : upto, over ? first : 31));
+        open &= over ? 0xfffffffeu << first : 0u;
+      }
+      if (r < p.rows) offset[r] = at;
+    }
+  }
   __syncthreads();
   // A thread writes up to four pages of its row, a warp longer rows in turn (a warp per row: 1024 rows with two new pages each 20.4 us,
-  // 64 rows 4.3; so 5.5 and 3.5).
+  // 64 rows 4.3; so 5.9 and 4.0, and 22.6 and 6.5 from a pool that is short by half).
   constexpr int kFewPages = 4;
   const int lane = threadIdx.x & 31;
   const auto give = [&](int r, int have, int at, int k) {
@@ -164,10 +194,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) allocate_kernel(PoolParams p,
     int have = 0, need = 0, at = 0;
     if (r < p.rows) {
       have = pages_of(p.seq_lens[r], p.page_size);
-      const int want = pages_of(new_lens[r], p.page_size);
+      need = demand(r);
       at = offset[r];
-      if (want <= p.width && want > have) need = want - have;
-      if (need > 0 && int64_t(at) + need > found) {
+      if (need > 0 && at < 0) {
         report(p.status, kPoolOutOfPages, r);
         need = 0;
       }

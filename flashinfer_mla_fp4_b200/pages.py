@@ -114,7 +114,8 @@ class FP4MLAPagePool:
     def allocate(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor) -> None:
         """Give each row the pages that ``new_lens`` (int32 [rows]) tokens take beyond those for ``seq_lens``; the lengths stay as they are.
 
-        Rows are served in order.  One that no longer fits into the pool, or into its block-table row, gets nothing."""
+        Rows are served in order.  One that no longer fits into the pool, or into its block-table row, gets nothing, and what there is stays for
+        the rows behind it."""
         if self._native(0, block_tables, seq_lens, new_lens) is not None:
             return
         check_tables(block_tables, seq_lens, self.device)

@@ -335,7 +335,8 @@ int mla_fp4_select_pages(const MlaFp4SelectArgs* args);
      mla_fp4_copy_pages: page src[i] to page dst[i] in every layer, i < count; pairs with a page outside the pool are skipped.  No page
        may be named twice among dst, or both in src and in dst: the copies run at once.
      mla_fp4_pool_allocate: pages for the rows that are to hold new_lens [rows] tokens and have those for seq_lens.  seq_lens stays as
-       it is.  Rows are served in order; one that does not fit any more, or not into its block-table row, gets none.
+       it is.  Rows are served in order; one that does not fit any more, or not into its block-table row, gets none and takes nothing
+       from the rows behind it.
      mla_fp4_pool_fork: row children[i] (empty: length 0) becomes what row parents[i] is, i < count.  Full pages are shared, a last page that is
        not full is copied in every layer.  A fork without a page for its tail, into a row that is not empty, or of a child named before, is not made.
      mla_fp4_pool_free: the rows' pages lose a reference each, their lengths become 0.

@@ -105,10 +105,10 @@ class Pool:
                 held[r] = n if want == have else self.sl[r]
                 continue
             got = free[at:at + want - have]
-            at += want - have
-            if len(got) < want - have:
+            if len(got) < want - have:  # (what there is stays for the rows behind it)
                 self.trouble = True
                 continue
+            at += want - have
             for k, p in enumerate(got):
                 self.bt[r][have + k] = p
                 self.ref[p] = 1

@@ -12,3 +12,9 @@ def test_ties_of_the_oracle():
     for q, scale in ((torch.zeros(1, 1, 2, 576), ssf), (torch.randn(1, 1, 2, 576), ssf * float("nan"))):
         got, lens = S.select(q.to(E4M3), summary, scale, bt, torch.tensor([2397]), 8, 40, 1, 2, False)
         assert got.tolist() == [bt[0, :38].tolist() + bt[0, -2:].tolist()] and lens.tolist() == [317]
+
+
+def test_oracle_allocation_from_a_pool_that_is_short():
+    p = S.Pool([0, 0, 1, 0, 0, 0], [[-1] * 9 for _ in range(5)], [0] * 5, 8)
+    assert p.allocate([64, 8, 16, 32, 16]) == [0, 8, 16, 0, 16] and p.trouble
+    assert [r[:2] for r in p.bt] == [[-1, -1], [0, -1], [1, 3], [-1, -1], [4, 5]] and p.ref == [1] * 6
