@@ -457,11 +457,11 @@ MlaFp4SelectArgs select_args(const at::Tensor& q, const at::Tensor& su, const at
   return s;
 }
 
-// select(q, summary, summary_sf, block_tables, seq_lens, page_size, budget, sink_pages, local_pages, causal, selected, selected_lens, workspace)
+// select(q, summary, summary_sf, block_tables, seq_lens, page_size, budget, sink_pages, local_pages, causal, selected, selected_lens, workspace, status)
 // -> (selected, selected_lens), or None when the call is not of the common form
 PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 13) return PyErr_Format(PyExc_TypeError, "select takes 13 arguments");
+  if (n != 14) return PyErr_Format(PyExc_TypeError, "select takes 14 arguments");
   const at::Tensor *q = tensor(a[0]), *su = tensor(a[1]), *ssf = tensor(a[2]), *bt = tensor(a[3]), *sl = tensor(a[4]);
   int64_t page;
   Budget b;
@@ -476,6 +476,8 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!t) Py_RETURN_NONE;
     out[i] = *t;
   }
+  const at::Tensor* st = a[13] == Py_None ? nullptr : tensor(a[13]);
+  if (a[13] != Py_None && (!st || !plain(*st, at::kInt, {8}, dev))) Py_RETURN_NONE;
   size_t need = 0;
   if (q->size(0) > INT32_MAX || q->size(1) > INT32_MAX || page < 0 || page > 128 ||
       abi.select_workspace_bytes(int32_t(q->size(0)), int32_t(q->size(1)), int32_t(width), &need) != MLA_FP4_OK)
@@ -486,6 +488,7 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   c10::cuda::CUDAGuard guard(dev);
   MlaFp4SelectArgs s = select_args(*q, *su, *ssf, *bt, *sl, page, b);
+  s.status = st ? static_cast<int32_t*>(st->data_ptr()) : nullptr;
   s.stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   int rc;
   {

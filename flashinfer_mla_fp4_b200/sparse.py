@@ -144,16 +144,17 @@ def summarize_new_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summa
 def select_pages(q: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                  page_size: int, budget_pages: int, *, sink_pages: int = 1, local_pages: int = 2, causal: bool = False,
                  selected: Optional[torch.Tensor] = None, selected_lens: Optional[torch.Tensor] = None,
-                 workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                 workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The pages that each query position attends to: ``(selected, selected_lens)``, int32 [batch * q_len, budget_pages] and
     [batch * q_len], a block table and lengths for a decode step of batch * q_len requests of one query position.
 
     ``q`` e4m3 [batch, q_len, H, 576] (strides that are multiples of 16, unit inner stride, H <= 128); ``seq_lens`` int32 [batch].  With ``causal``
     position i of q_len does not see the q_len - 1 - i newest tokens; without it every position sees all of them, as in
     ``BatchMLADecodeCuteDSLFP4Wrapper.run``.  Entries behind a row's last page are 0.  ``workspace`` (int8, ``4 * batch * q_len`` times
-    max_pages rounded up to a multiple of four; 16-byte aligned; allocated when not given) holds the scores.  Asynchronous on the current stream, capturable."""
+    max_pages rounded up to a multiple of four; 16-byte aligned; allocated when not given) holds the scores.  ``status`` (int32 [8], zeroed) gets the error of
+    a device-side wait that ran out: the pages are then some of the request's, but not the best.  Asynchronous on the current stream, capturable."""
     done = _native.select(q, summary, summary_sf, block_tables, seq_lens, page_size, budget_pages, sink_pages, local_pages, causal,
-                          selected, selected_lens, workspace)
+                          selected, selected_lens, workspace, status)
     if done is not None:
         return done
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[-1] != HEAD_DIM_QK or q.dtype != torch.float8_e4m3fn:
@@ -187,6 +188,8 @@ def select_pages(q: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tenso
         check_tensor("workspace", workspace, torch.int8, (None,), dev)
         if workspace.numel() < need:
             raise ValueError(f"workspace has {workspace.numel()} bytes, but {need} are required")
+    if status is not None:
+        check_tensor("status", status, torch.int32, (8,), dev)
     if rows == 0:
         return selected, selected_lens
     a = _cabi.SelectArgs()
@@ -198,6 +201,7 @@ def select_pages(q: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tenso
     a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
     a.batch, a.q_len, a.num_heads, a.page_size, a.width = batch, q_len, heads, page_size, width
     a.budget, a.sink_pages, a.local_pages, a.causal = budget_pages, sink_pages, local_pages, 1 if causal else 0
+    a.status = None if status is None else status.data_ptr()
     with torch.cuda.device(dev):
         a.stream = torch.cuda.current_stream(dev).cuda_stream
         _cabi.check(_cabi.lib.mla_fp4_select_pages(C.byref(a)))
@@ -280,7 +284,7 @@ class BatchMLASparseDecodeFP4Wrapper:
         rows = batch * q_len
         selected, selected_lens, scores = self._scratch(rows, width)
         select_pages(q, summary, summary_sf, block_tables, seq_lens, page_size, sp.budget_pages, sink_pages=sp.sink_pages,
-                     local_pages=sp.local_pages, causal=sp.causal, selected=selected, selected_lens=selected_lens, workspace=scores)
+                     local_pages=sp.local_pages, causal=sp.causal, selected=selected, selected_lens=selected_lens, workspace=scores, status=dense._status)
         got = self._dense.run(q.as_strided((rows, 1, heads, HEAD_DIM_QK), (q.stride(0) if q_len == 1 else q.stride(1), 16, q.stride(2), 1)), kv_cache,
                               selected, selected_lens, min(max_seq_len, sp.budget_pages * page_size), softmax_scale, output_scale,
                               out=None if out is None else out.view(rows, 1, heads, -1), kv_cache_sf=kv_cache_sf, return_lse=return_lse,

@@ -94,6 +94,75 @@ def test_the_first_record_of_a_wait_that_ran_out_stays():
     assert slow.run(1, before) == before
 
 
+_BOUND = ("mla_fp4_summarize_pages", "mla_fp4_summarize_new_pages", "mla_fp4_select_workspace_bytes", "mla_fp4_select_pages",
+          "mla_fp4_pool_workspace_bytes", "mla_fp4_pool_allocate", "mla_fp4_pool_fork", "mla_fp4_pool_free", "mla_fp4_pool_compact")
+
+
+@pytest.fixture
+def one_poll(monkeypatch):
+    """Selections with a poll budget of one, whichever way the library is called."""
+    from flashinfer_mla_fp4_b200 import _cabi
+
+    _dev()
+    real = _cabi.lib.mla_fp4_select_pages
+
+    def with_one_poll(args):
+        a = args.contents if hasattr(args, "contents") else args._obj
+        a.wait_polls = 1
+        return real(C.byref(a))
+
+    stand_in = C.CFUNCTYPE(C.c_int, C.POINTER(_cabi.SelectArgs))(with_one_poll)
+    addresses = {n: C.cast(getattr(_cabi.lib, n), C.c_void_p).value for n in _BOUND}
+    monkeypatch.setattr(_cabi.lib, "mla_fp4_select_pages", with_one_poll)
+    _cabi.native.bind_sparse(*{**addresses, "mla_fp4_select_pages": C.cast(stand_in, C.c_void_p).value}.values())
+    yield
+    _cabi.native.bind_sparse(*addresses.values())
+
+
+class _Decline:
+    """A native call path that leaves every call to the Python one."""
+
+    def __getattr__(self, name):
+        return lambda *args: False if name == "summarize" else None
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_select_pages_reports_a_wait_that_ran_out(native, monkeypatch, request):
+    slow = _Slow()  # (before the poll budget is cut)
+    request.getfixturevalue("one_poll")
+    from flashinfer_mla_fp4_b200 import _cabi, sparse
+
+    if not native:
+        monkeypatch.setattr(sparse, "_native", _Decline())
+    slow.cold.fill_(1)
+    got, lens = sparse.select_pages(*slow.inputs, 64, 64, status=slow.status)
+    torch.cuda.synchronize()
+    assert int(slow.status[0]) == _cabi.ERR_DEVICE_TIMEOUT and torch.equal(lens, slow.want[1])
+    for wrong in (slow.status[:7], slow.status.long(), slow.status.cpu(), torch.zeros(16, dtype=torch.int32, device=slow.bt.device)[::2]):
+        with pytest.raises(ValueError, match="status"):
+            sparse.select_pages(*slow.inputs, 64, 64, status=wrong)
+
+
+@pytest.mark.parametrize("validate", ["0", "1"])
+def test_a_sparse_step_reports_a_wait_of_its_selection(validate, monkeypatch, request):
+    """Also when the page ids are checked on the host first, which the native call leaves to the Python one."""
+    slow = _Slow()
+    request.getfixturevalue("one_poll")
+    from flashinfer_mla_fp4_b200 import BatchMLASparseDecodeFP4Wrapper
+
+    monkeypatch.setenv("MLA_FP4_VALIDATE", validate)
+    q, summary, ssf, bt, sl = slow.inputs
+    dev, pages = q.device, summary.shape[0]
+    kv, sf = torch.zeros(pages, 64, 320, dtype=torch.uint8, device=dev), torch.ones(pages, 64, 1, device=dev)
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    w = BatchMLASparseDecodeFP4Wrapper(torch.empty(BatchMLASparseDecodeFP4Wrapper.workspace_bytes(124, 1, 128, 2048, 64, sms), dtype=torch.int8, device=dev))
+    w.plan(num_heads=128, page_size=64, budget_pages=64)
+    slow.cold.fill_(1)
+    w.run(q, kv, bt, sl, 2048 * 64, 0.04, kv_cache_sf=sf, summary=summary, summary_sf=ssf)
+    with pytest.raises(RuntimeError):
+        w.check_device_status()
+
+
 def _one_sided_pages(page):
     """Pages one part of whose summary is nothing beside the other: the factor that takes a sum to a code is beyond FP32 where the sums are all zero."""
     kv, sf = _pages(12, page, page + 7)
