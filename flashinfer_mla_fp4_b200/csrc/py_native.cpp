@@ -435,6 +435,7 @@ struct Budget {
   // from four Python values; false: not of the common form
   bool from(PyObject* const* a) {
     causal = PyObject_IsTrue(a[3]);
+    if (causal < 0) PyErr_Clear();  // (the Python path says what is wrong with it)
     return integer(a[0], &budget) && integer(a[1], &sink) && integer(a[2], &local) && causal >= 0 && sink >= 0 && local >= 1 && sink <= INT32_MAX &&
            local <= INT32_MAX && budget <= INT32_MAX && sink + local <= budget;
   }

@@ -169,6 +169,7 @@ def select_pages(q: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tenso
         raise ValueError(f"Unsupported page_size={page_size}: must be one of {PAGE_SIZES}")
     if q_len < 1 or not 1 <= heads <= 128:
         raise ValueError(f"q must have at least one query position and 1 to 128 heads, got {tuple(q.shape)}")
+    causal = bool(causal)
     SparsePages(budget_pages, sink_pages, local_pages)  # (its checks)
     pages = check_summary(summary, summary_sf, None, dev)
     check_tables(block_tables, seq_lens, dev, batch)
@@ -200,7 +201,7 @@ def select_pages(q: torch.Tensor, summary: torch.Tensor, summary_sf: torch.Tenso
     a.selected, a.selected_lens = selected.data_ptr(), selected_lens.data_ptr()
     a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
     a.batch, a.q_len, a.num_heads, a.page_size, a.width = batch, q_len, heads, page_size, width
-    a.budget, a.sink_pages, a.local_pages, a.causal = budget_pages, sink_pages, local_pages, 1 if causal else 0
+    a.budget, a.sink_pages, a.local_pages, a.causal = budget_pages, sink_pages, local_pages, int(causal)
     a.status = None if status is None else status.data_ptr()
     with torch.cuda.device(dev):
         a.stream = torch.cuda.current_stream(dev).cuda_stream

@@ -163,6 +163,15 @@ def test_a_sparse_step_reports_a_wait_of_its_selection(validate, monkeypatch, re
         w.check_device_status()
 
 
+def test_a_causal_that_is_neither_true_nor_false_is_refused():
+    _dev()
+    from flashinfer_mla_fp4_b200.sparse import select_pages
+
+    args = [t.cuda() for t in _selection_case([700], 8, 16, 1, seed=2)]
+    with pytest.raises((ValueError, RuntimeError), match="ambiguous"):
+        select_pages(*args, 16, 8, causal=torch.tensor([True, False]))
+
+
 def _one_sided_pages(page):
     """Pages one part of whose summary is nothing beside the other: the factor that takes a sum to a code is beyond FP32 where the sums are all zero."""
     kv, sf = _pages(12, page, page + 7)
