@@ -32,6 +32,7 @@ from .kvcache import HEAD_DIM_QK, ROW_BYTES
 from .wrapper import BatchMLADecodeCuteDSLFP4Wrapper, validate_page_ids
 
 PAGE_SIZES = (8, 16, 32, 64, 128)
+_INT32 = 2**31 - 1  # counts are handed to the kernels in 32 bits
 _native = _cabi.native
 
 
@@ -45,6 +46,8 @@ class SparsePages:
     causal: bool = False
 
     def __post_init__(self) -> None:
+        if self.budget_pages > _INT32:
+            raise ValueError(f"budget_pages must be below 2^31, got {self.budget_pages}")
         if self.sink_pages < 0 or self.local_pages < 1 or self.sink_pages + self.local_pages > self.budget_pages:
             raise ValueError(f"sink_pages ({self.sink_pages}) must not be negative, local_pages ({self.local_pages}) at least 1, and their "
                              f"sum within budget_pages ({self.budget_pages})")
@@ -64,6 +67,8 @@ def check_tables(block_tables, seq_lens, device, batch: Optional[int] = None) ->
     if not isinstance(block_tables, torch.Tensor) or block_tables.dtype != torch.int32 or block_tables.dim() != 2 or (
             block_tables.shape[1] > 0 and block_tables.stride(1) != 1) or block_tables.stride(0) < 0:
         raise ValueError("block_tables must be an int32 [batch, max_pages] tensor with unit inner stride")
+    if max(block_tables.shape) > _INT32:
+        raise ValueError(f"block_tables must have fewer than 2^31 rows and pages a row, got {tuple(block_tables.shape)}")
     if not block_tables.is_cuda or block_tables.device != device:
         raise ValueError(f"block_tables must be a CUDA tensor on {device}, got {block_tables.device}")
     if batch is not None and block_tables.shape[0] != batch:
@@ -136,7 +141,7 @@ def summarize_new_pages(kv_cache: torch.Tensor, kv_cache_sf: torch.Tensor, summa
     with torch.cuda.device(dev):
         _cabi.check(_cabi.lib.mla_fp4_summarize_new_pages(
             kv_cache.data_ptr(), kv_cache_sf.data_ptr(), pages, page_size, block_tables.data_ptr(), block_tables.stride(0), width,
-            seq_lens.data_ptr(), batch, min(int(new_tokens), 2**31 - 1), summary.data_ptr(), summary_sf.data_ptr(),
+            seq_lens.data_ptr(), batch, min(int(new_tokens), _INT32), summary.data_ptr(), summary_sf.data_ptr(),
             None if status is None else status.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
 
 

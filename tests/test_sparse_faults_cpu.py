@@ -31,3 +31,17 @@ def test_a_causal_that_is_neither_true_nor_false_is_no_internal_error(causal):
     bt, sl = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):  # (what is wrong with these tensors otherwise)
         select_pages(q, summary, ssf, bt, sl, 16, 4, causal=causal)
+
+
+def test_counts_beyond_32_bits_are_refused():
+    """They would be cut to their low bits on their way to the kernels: a budget of 2^32 + 8 would be one of 8."""
+    from flashinfer_mla_fp4_b200 import SparsePages
+    from flashinfer_mla_fp4_b200.sparse import check_tables
+
+    assert SparsePages(2**31 - 1).budget_pages == 2**31 - 1
+    for budget in (2**31, 2**32 + 8):
+        with pytest.raises(ValueError, match="2\\^31"):
+            SparsePages(budget)
+    for shape in ((1, 2**31), (2**31, 1)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            check_tables(torch.empty(shape, dtype=torch.int32, device="meta"), None, torch.device("cuda:0"))
