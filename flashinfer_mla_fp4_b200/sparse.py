@@ -232,7 +232,8 @@ class BatchMLASparseDecodeFP4Wrapper:
     def plan(self, num_heads: int, page_size: int, budget_pages: int, sink_pages: int = 1, local_pages: int = 2, causal: bool = False,
              out_dtype: Optional[torch.dtype] = None, variant=None, enable_pdl: Optional[bool] = None, max_ctas: Optional[int] = None) -> None:
         """Validate and bind the configuration.  ``causal``: position i of q_len does not see the q_len - 1 - i newest tokens.  The other
-        arguments are those of ``SparsePages`` and of the dense wrapper's ``plan``."""
+        arguments are those of ``SparsePages`` and of the dense wrapper's ``plan``; ``max_ctas`` caps the attention's grid and with it the partials, not
+        the selection's, which takes up to two CTAs an SM for the scores and one a query position after them."""
         pages = SparsePages(budget_pages, sink_pages, local_pages, bool(causal))
         self._dense.plan(num_heads=num_heads, page_size=page_size, out_dtype=out_dtype, variant=variant, enable_pdl=enable_pdl, max_ctas=max_ctas)
         self._pages, self._num_heads, self._page_size = pages, num_heads, page_size

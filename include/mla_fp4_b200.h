@@ -336,7 +336,8 @@ int mla_fp4_select_pages(const MlaFp4SelectArgs* args);
        may be named twice among dst, or both in src and in dst: the copies run at once.
      mla_fp4_pool_allocate: pages for the rows that are to hold new_lens [rows] tokens and have those for seq_lens.  seq_lens stays as
        it is.  Rows are served in order; one that does not fit any more, or not into its block-table row, gets none and takes nothing
-       from the rows behind it.
+       from the rows behind it.  The caller takes the new lengths over into seq_lens before its next call on the pool: until then no row has the new
+       pages (free or a second allocate would lose them, compact would leave their table entries on the old numbers).
      mla_fp4_pool_fork: row children[i] (empty: length 0) becomes what row parents[i] is, i < count.  Full pages are shared, a last page that is
        not full is copied in every layer.  A fork without a page for its tail, into a row that is not empty, or of a child named before, is not made.
      mla_fp4_pool_free: the rows' pages lose a reference each, their lengths become 0.
