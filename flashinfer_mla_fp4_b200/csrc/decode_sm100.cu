@@ -1945,14 +1945,16 @@ cudaError_t launch_decode_sm100(const DecodeParams& p, int num_ctas, cudaStream_
   cfg.dynamicSmemBytes = kSmemAlloc;
   cfg.stream = stream;
   // Programmatic dependent launch: the CTAs are placed and run their prologue while the kernel before this one on the
-  // stream drains, then wait for that kernel's completion.
+  // stream drains, then wait for that kernel's completion.  Not with more requests than a plan has room for: it reads the lengths of the others twice, and
+  // between the two the kernel before may write them (were all tiles gone the second time, the walk would look for them for ever).
+  const bool early = p.pdl && p.batch <= kLensMax;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.pdl ? 1 : 0;
+  cfg.numAttrs = early ? 1 : 0;
   DecodeParams pp = p;
-  pp.pdl_wait = p.pdl;
+  pp.pdl_wait = early;
   pp.page_shift = __builtin_ctz(unsigned(p.page_size));
   return cudaLaunchKernelEx(&cfg, kernel, pp, map_q_lat, map_q_rope, map_rope, map_lat);
 }

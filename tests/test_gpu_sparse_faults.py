@@ -4,7 +4,8 @@ import ctypes as C
 import pytest
 import torch
 
-from test_gpu_sparse import E4M3, _dev, _oracle_summaries, _pages, _same, _selection_case
+from oracle import mla_fp4_oracle as O
+from test_gpu_sparse import E4M3, _dev, _oracle_summaries, _pages, _same, _selection_case, _sparse_case, _wrapper
 
 pytestmark = pytest.mark.gpu
 
@@ -170,6 +171,29 @@ def test_a_causal_that_is_neither_true_nor_false_is_refused():
     args = [t.cuda() for t in _selection_case([700], 8, 16, 1, seed=2)]
     with pytest.raises((ValueError, RuntimeError), match="ambiguous"):
         select_pages(*args, 16, 8, causal=torch.tensor([True, False]))
+
+
+def test_more_requests_than_a_plan_holds_whose_lengths_come_and_go():
+    """Lengths that the kernel ahead of the decode writes in every step, from tokens to none and back: a plan must not be made from both."""
+    cache, _, _, _ = _sparse_case([64], 8, 8, 1, seed=2)
+    dev, rows = cache.kv_cache.device, 20600
+    bt = (torch.arange(rows, device=dev) % 8).int().view(rows, 1).repeat(1, 2).contiguous()
+    q = torch.randn(1, 1, 8, 576, generator=torch.Generator().manual_seed(3)).to(E4M3).to(dev).expand(rows, 1, 8, 576)
+    w = _wrapper(num_heads=8, page_size=8, budget_pages=3)
+    some = torch.zeros(rows, dtype=torch.int32, device=dev)
+    some[20500:] = 5
+    every, none, sl = torch.full_like(some, 5), torch.zeros_like(some), torch.zeros_like(some)
+    want = None
+    for i in range(60):
+        lens = (every, none, some, none)[i % 4]
+        sl.copy_(lens)
+        out = w.run(q, cache.kv_cache, bt, sl, 16, 0.05, kv_cache_sf=cache.kv_cache_sf, summary=cache.summary, summary_sf=cache.summary_sf)
+        want = out.clone() if want is None else want
+        assert torch.equal(out, torch.where((lens > 0).view(rows, 1, 1, 1), want, torch.zeros_like(want)))
+    w.check_device_status()
+    ref, _ = O.mla_decode(q[:8].cpu(), cache.kv_cache, cache.kv_cache_sf, bt[:8].cpu(), every[:8].cpu(), 0.05)
+    O.assert_parity(want[:8].float().cpu(), ref, "the first requests")
+    assert torch.equal(want, want[:8].repeat(rows // 8, 1, 1, 1))
 
 
 def _one_sided_pages(page):
