@@ -149,8 +149,8 @@ __global__ void __launch_bounds__(kSumThreads) summarize_kernel(SummarizeParams 
     const float scale = unsound_s ? CUDART_NAN_F : summary_scale(ml, mr, top, kLatUnit, kRopeUnit);
     if (lane == 0) {
       scale_s = scale;
-      by_s[0] = top / scale * float(kLatUnit);
-      by_s[1] = float(kRopeUnit) / scale;
+      by_s[0] = summary_factor(top / scale * float(kLatUnit));
+      by_s[1] = summary_factor(float(kRopeUnit) / scale);
     }
   }
   __syncthreads();
@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(kSumThreads) summarize_four_kernel(SummarizePa
     const float scale = unsound_s[sub] ? CUDART_NAN_F : summary_scale(max(most_s[sub][0], most_s[sub][1]), most_rope, top, kLatUnit, kRopeUnit);
     if (lane == 0) {
       scale_s[sub] = scale;
-      by_s[sub][0] = top / scale * float(kLatUnit);
-      by_s[sub][1] = float(kRopeUnit) / scale;
+      by_s[sub][0] = summary_factor(top / scale * float(kLatUnit));
+      by_s[sub][1] = summary_factor(float(kRopeUnit) / scale);
       if (there) p.summary_sf[page] = scale;
     }
   }

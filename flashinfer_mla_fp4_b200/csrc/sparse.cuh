@@ -99,10 +99,12 @@ __device__ __forceinline__ float summary_scale(int most_lat, int most_rope, floa
   const double off = fma(-127.0, double(q), largest);  // q is the nearest but for the rounding of the product
   return off > 63.5 * double(up - q) ? up : off < -63.5 * double(q - down) ? down : q;
 }
+// What takes a sum to its code, kept finite: beside a part of the page that outweighs it beyond FP32 it would be infinite, and infinity times a sum of zero
+// NaN.  No other sum meets a factor that large: the scale is at least |sum| * top * unit / 127, or half that where it is subnormal.
+__device__ __forceinline__ float summary_factor(float by) { return fminf(by, __uint_as_float(0x7f7fffffu)); }
 // round(sum * top * unit / scale), within [-127, 127]; 0 where the scale is 0 or NaN.  `by` is top * unit / scale in FP32, and will do unless the
 // product is too near the middle of two whole numbers (it is off by less than 2^-14: roundings of 5 * 127 half-ulps of 1): then the
-// sum is compared with the middle in 64 bits.  A sum of 0 is code 0 whatever `by` is: beside a part of the page that outweighs it beyond FP32, `by` may be
-// infinite, which no other sum can meet (the scale is at least |sum| * top * unit / 127, and half that where it is subnormal).
+// sum is compared with the middle in 64 bits.
 __device__ __forceinline__ int summary_code(int sum, float scale, float by, float top, double unit) {
   const float x = float(sum) * by;
   float whole = rintf(x);
@@ -112,7 +114,7 @@ __device__ __forceinline__ int summary_code(int sum, float scale, float by, floa
     const float toward = copysignf(0.5f, x);
     whole = over == 0.0 ? rintf(middle) : (over > 0.0) == (x > 0.f) ? middle + toward : middle - toward;
   }
-  return scale > 0.f && sum != 0 ? int(fminf(fmaxf(whole, -127.f), 127.f)) : 0;
+  return scale > 0.f ? int(fminf(fmaxf(whole, -127.f), 127.f)) : 0;
 }
 
 // what a bounded wait that ran out leaves in the status words: the first one's record, as in the decode kernel

@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1) summarize_many_kernel(SummarizePa
         float scale = summary_scale(ml, mr, top, kLatUnit, kRopeUnit);
         if (!(top <= CUDART_MAX_NORMAL_F) || mr >= kRopeNan / 2) scale = CUDART_NAN_F;
         g.scale[t] = scale;
-        g.by_lat[t] = top / scale * float(kLatUnit);
-        g.by_rope[t] = float(kRopeUnit) / scale;
+        g.by_lat[t] = summary_factor(top / scale * float(kLatUnit));
+        g.by_rope[t] = summary_factor(float(kRopeUnit) / scale);
         if (s.page[b][t] >= 0) p.summary_sf[s.page[b][t]] = scale;
       }
       ptx::bar_sync(2 + group, 128);
