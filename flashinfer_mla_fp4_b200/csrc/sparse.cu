@@ -474,11 +474,11 @@ __global__ void __launch_bounds__(kSelMost) select_kernel(SelectParams p) {
 // Which kernel, us in graphs of calls on pages that are not in L2, for 4096 / 38000 / 150000 / 300000 tokens (a CTA per page, four pages a CTA, many):
 //   pages of   8   3.6 / 16.8 / 59.5 / 116     3.4 /  9.0 / 26.5 / 50.1    (sixteen pages to a tile) 12 / 25 / 65 / 120
 //             16   3.7 / 10.4 / 33.5 / 64.3    3.2 /  7.9 / 21.2 / 38.3    (eight) 8.3 / 16.2 / 38.8 / 73.4
-//             32   3.0 /  7.4 / 21.3 / 39.6    3.9 /  9.7 / 18.7 / 33.0    6.4 / 10.0 / 19.5 / 32.5
-//             64   3.1 /  6.6 / 18.3 / 32.6    5.3 /  9.7 / 17.2 / 29.0    5.2 /  8.3 / 16.6 / 26.3
-//            128   3.5 /  6.4 / 17.0 / 28.2    8.4 / 11.2 / 22.6 / 30.3    4.9 /  7.3 / 15.6 / 24.2
+//             32   3.0 /  7.4 / 21.3 / 39.6    3.9 /  9.7 / 18.7 / 33.0    6.4 / 10.0 / 18.4 / 31.2
+//             64   3.1 /  6.6 / 18.3 / 32.6    5.3 /  9.7 / 17.2 / 29.0    5.2 /  8.3 / 15.5 / 25.0
+//            128   3.5 /  6.4 / 17.0 / 28.2    8.4 / 11.2 / 22.6 / 30.3    4.9 /  7.3 / 14.1 / 22.4
 // With small pages what is done once a page outweighs its sums, and four share it; with large ones four in turn are longer than one by four groups.
-constexpr int64_t kManyTokens = 131072;  // (76000: 11.1 with a CTA per page, 11.8)
+constexpr int64_t kManyTokens = 131072;  // of a call's places for pages (76000: 11.1 with a CTA per page, 11.8)
 
 cudaError_t launch_summarize(const SummarizeParams& p, int64_t count, int sms, cudaStream_t stream) {
   if (p.page_size <= 16) {

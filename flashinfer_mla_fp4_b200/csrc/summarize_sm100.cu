@@ -8,7 +8,7 @@
 //
 // Bound by the copies: 324 bytes a token from HBM, of which the latent comes in pieces of 64 bytes; a tile takes 2300 to 2450 clk, as in the
 // decode kernel, where its bytes at the measured rate would take 1800.  What the other kernel spends on taking codes apart (two pages of 64
-// tokens: some 8000 warp instructions at 3 a clk) is done by 16 MMAs.  8192 pages of 64 tokens: 54 us there, 43.7 here, floor 26.5.
+// tokens: some 8000 warp instructions at 3 a clk) is done by 16 MMAs.  8192 pages of 64 tokens: 54 us there, 39.0 here, floor 27.2.
 //
 // Roles: warp 0 TMA, warp 1 MMAs, warps 4-7 (front) weights and RoPE sums, warps 8-15 (back) sums out of TMEM, scales, codes; the two
 // groups of the back take the tiles in turn (one group: 2900 clk a tile).  Scales and RoPE bytes come with the tile (read by the
