@@ -117,7 +117,7 @@ class FP4MLAPagePool:
         Rows are served in order.  One that no longer fits into the pool, or into its block-table row, gets nothing, and what there is stays for
         the rows behind it.  Take the new lengths over into ``seq_lens`` before the next call on the pool: until then no row has the new pages, so
         ``free`` or a second ``allocate`` would lose them, ``fork`` would not share them and ``compact`` would leave their table entries on the old numbers.  A length may
-        be lowered within the row's last page; a page behind the new end would be the row's no longer, and nobody's."""
+        be lowered within the row's last page if no fork shares that (a full one may be shared); a page behind the new end would be the row's no longer, and nobody's."""
         if self._native(0, block_tables, seq_lens, new_lens) is not None:
             return
         check_tables(block_tables, seq_lens, self.device)

@@ -338,7 +338,7 @@ int mla_fp4_select_pages(const MlaFp4SelectArgs* args);
        it is.  Rows are served in order; one that does not fit any more, or not into its block-table row, gets none and takes nothing
        from the rows behind it.  The caller takes the new lengths over into seq_lens before its next call on the pool: until then no row has the new
        pages (free or a second allocate would lose them, compact would leave their table entries on the old numbers).
-       Nor has a row the pages behind its end when its length is lowered: lengths may be lowered within the last page.
+       Nor has a row the pages behind its end when its length is lowered: lengths may be lowered within the last page, if no fork shares it.
      mla_fp4_pool_fork: row children[i] (empty: length 0) becomes what row parents[i] is, i < count.  Full pages are shared, a last page that is
        not full is copied in every layer.  A fork without a page for its tail, into a row that is not empty, or of a child named before, is not made.
      mla_fp4_pool_free: the rows' pages lose a reference each, their lengths become 0.
